@@ -1,0 +1,469 @@
+// Attention of a step's tokens over the paged cache where the requests of a group share a long prefix: its keys and values
+// are read once for all tokens of the group, a token's own keys behind it for that token.
+//   token t of group g, at position p:  out = sum_j softmax_j(scale q.k_j) v_j  over the keys j <= p; of these,
+//   j < shared_g lie in the pages that the group's first request names, the others in those of the token's own request.
+// A softmax over parts of the keys joins exactly: with (m, l, O) = (max, sum exp(s - m), sum exp(s - m) v) of each part and
+// M the largest m, out = sum exp(m - M) O / sum exp(m - M) l.
+//
+// Two launches.  The first makes the prefixes' parts: an item is (group, key head, some rows), a row a (token, query head of
+// that key head), so keys serve rows from shared memory; the tiles of keys of all items, one after the other, are dealt to
+// the blocks in equal shares, so a block's share may end inside an item and every block has the same work, whatever the
+// lengths.  What a block finds for (a piece of) an item goes to the workspace.  The second launch makes the tokens' own parts,
+// which it does while the first still runs, waits for that, and joins all parts of a (token, head).
+#include "attention_prefix.cuh"
+
+SGLC_DEFINE_ERROR_STRING()
+
+namespace {
+using namespace prefix;
+
+// ---- prefixes, 32-bit arithmetic (any head size that is a multiple of 8, up to 256) -----------------------------------------
+// A tile of 64 rows by 64 keys: a thread has 4 x 4 scores, fed by 16-byte reads of queries and keys from shared memory (8 for
+// 64 multiply-adds), and 4 rows by D / 16 columns of the sums.
+constexpr int GT = 256;                   // threads
+constexpr int GR = GENERAL_ROWS, GK = GENERAL_KEYS;
+
+template <typename T, int NC>             // NC: blocks of 64 columns
+__global__ void __launch_bounds__(GT)
+prefix_general_kernel(const Args a) {
+  extern __shared__ __align__(16) float sm[];
+  const int D = a.D, DS = D + 4;          // (rows of queries and keys four words apart from the banks' period)
+  float* sQ = sm;                         // [GR][DS]
+  float* sK = sQ + GR * DS;               // [GK][DS]
+  float* sV = sK + GK * DS;               // [GK][NC * 64]
+  float* sP = sV + GK * NC * 64;          // [GR][GK + 4]
+  __shared__ Plan plan;
+  __shared__ int lim[GR];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  pdl_wait();
+  pdl_launch_dependents();                // (here and not before: the second launch reads what came before this one)
+  make_plan(a, plan);
+  const float c2 = a.scale * LOG2E;
+  const int gq = a.H / a.Hkv;
+  for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
+    const int row0 = s.row_tile * GR, rows = min(GR, s.n_rows - row0);
+    __syncthreads();
+    for (int x = tid; x < GR * (D / 8); x += GT) {
+      const int row = x / (D / 8), d = x % (D / 8) * 8;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = 0.0f;
+      if (row < rows) {
+        const int n = row0 + row, t = s.t0 + n / gq, h = s.hk * gq + n % gq;
+        load8(reinterpret_cast<const T*>(a.q) + (size_t)t * a.q_stride + (size_t)h * D + d, a.q_vec, v);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) sQ[row * DS + d + i] = v[i];
+    }
+    if (tid < GR) lim[tid] = tid < rows ? visible(a, s.t0 + (row0 + tid) / gq, s.keys) : 0;
+    float m[4], l[4], o[4][NC][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) o[i][c][u] = 0.0f;
+    }
+    for (int j = 0; j < s.tiles; j++) {
+      const int key0 = (s.tile + j) * GK;
+      __syncthreads();
+      for (int x = tid; x < GK * NC * 8; x += GT) {
+        const int row = x / (NC * 8), d = x % (NC * 8) * 8, key = key0 + row;
+        float k[8], v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) k[i] = v[i] = 0.0f;
+        if (d < D && key < s.keys) {
+          const int page = page_of(a, s.req, key);
+          if (page >= 0) {
+            const size_t at = row_at(a, page, s.hk, key) + d;
+            load8(reinterpret_cast<const T*>(a.cache) + at, 1, k);
+            load8(reinterpret_cast<const T*>(a.cache) + at + value_offset(a), 1, v);
+          }
+        }
+        if (d < D)
+#pragma unroll
+          for (int i = 0; i < 8; i++) sK[row * DS + d + i] = k[i];
+#pragma unroll
+        for (int i = 0; i < 8; i++) sV[row * NC * 64 + d + i] = v[i];
+      }
+      __syncthreads();
+      float x[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[i][u] = 0.0f;
+      for (int d = 0; d < D; d += 4) {
+        float4 q4[4], k4[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) q4[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * DS + d]);
+#pragma unroll
+        for (int u = 0; u < 4; u++) k4[u] = *reinterpret_cast<const float4*>(&sK[(tx + 16 * u) * DS + d]);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            x[i][u] = fmaf(q4[i].x, k4[u].x, x[i][u]);
+            x[i][u] = fmaf(q4[i].y, k4[u].y, x[i][u]);
+            x[i][u] = fmaf(q4[i].z, k4[u].z, x[i][u]);
+            x[i][u] = fmaf(q4[i].w, k4[u].w, x[i][u]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int row = ty * 4 + i, n = lim[row] - key0;      // keys of this tile that the row sees
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          if (tx + 16 * u >= n) x[i][u] = -INFINITY;
+          mx = fmaxf(mx, x[i][u]);
+        }
+#pragma unroll
+        for (int w = 1; w < 16; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        mx *= c2;
+        if (mx > m[i]) {
+          const float f = exp2f(m[i] - mx);                   // (0 where nothing was seen before)
+          m[i] = mx;
+          l[i] *= f;
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) o[i][c][u] *= f;
+        }
+        const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const float p = exp2f(fmaf(x[i][u], c2, -ref));
+          l[i] += p;
+          sP[row * (GK + 4) + tx + 16 * u] = p;
+        }
+      }
+      __syncwarp();                       // (a row's weights are made and used by the same half of a warp)
+#pragma unroll 2
+      for (int key = 0; key < GK; key += 4) {
+        float4 p4[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) p4[i] = *reinterpret_cast<const float4*>(&sP[(ty * 4 + i) * (GK + 4) + key]);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          float4 v4[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) v4[u] = *reinterpret_cast<const float4*>(&sV[(key + u) * NC * 64 + c * 64 + tx * 4]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float w[4] = {p4[i].x, p4[i].y, p4[i].z, p4[i].w};
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+              o[i][c][0] = fmaf(w[u], v4[u].x, o[i][c][0]);
+              o[i][c][1] = fmaf(w[u], v4[u].y, o[i][c][1]);
+              o[i][c][2] = fmaf(w[u], v4[u].z, o[i][c][2]);
+              o[i][c][3] = fmaf(w[u], v4[u].w, o[i][c][3]);
+            }
+          }
+        }
+      }
+    }
+    const size_t slot = (size_t)(blockIdx.x + s.item) * a.slot_rows;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int row = ty * 4 + i;
+#pragma unroll
+      for (int w = 1; w < 16; w <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+      if (row < rows && slot_ok(a, s)) {
+        if (tx == 0) a.part_ml[slot + row] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+          if (c * 64 + tx * 4 < D)
+            *reinterpret_cast<float4*>(a.part_o + (slot + row) * D + c * 64 + tx * 4) =
+                make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+      }
+    }
+  }
+}
+
+// ---- a token's own keys, and the parts joined ------------------------------------------------------------------------------
+// A block has HC query heads of one key head of one token, or a share of their keys (a cluster of up to 8 blocks).  A key's
+// row is spread over the lanes of a part of a warp, eight entries a lane; each such part walks keys of its own with a running
+// maximum of its own.
+constexpr int OT = 128;
+
+template <typename T, int HC>
+__global__ void __launch_bounds__(OT)
+prefix_own_kernel(const Args a) {
+  extern __shared__ __align__(16) float sm[];
+  __shared__ Plan plan;
+  const int D = a.D, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = a.H / a.Hkv;
+  const int share = blockIdx.z, shares = gridDim.z;
+  const int chunks = a.H / HC, t = blockIdx.x / chunks, h0 = blockIdx.x % chunks * HC, hk = h0 / gq;
+  const int width = a.lanes, lanes_of = lane / width, sub = lane % width, walkers = OT / width;
+  float* part = sm;                                   // [walkers][HC][D + 2]: sums, then maximum and sum of weights
+  float* mine = part + walkers * HC * (D + 2);        // [HC][D + 2]: this block's
+  float* weight = mine + HC * (D + 2);                // [HC][prefix parts]
+  if (shares > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  pdl_launch_dependents();
+  make_plan(a, plan);
+  const int g = group_of(a, plan, t);
+  if (g < 0) {                                        // a token behind or before all groups (the whole cluster leaves)
+    pdl_wait();
+    return;
+  }
+  const float c2 = a.scale * LOG2E;
+  const int keys = plan.keys[g], pos = a.positions[t];
+  const int req = request_of(a, t);
+  const int n_all = min(pos, a.last_position) + 1, n_own = req < 0 ? 0 : max(0, n_all - keys);
+  if (pos > a.last_position && tid == 0 && share == 0) flag_index(a);
+  const int first = keys + (int)((long long)n_own * share / shares), last = keys + (int)((long long)n_own * (share + 1) / shares);
+  {
+    const int d = sub * 8;
+    float q[HC][8], m[HC], l[HC], o[HC][8];
+#pragma unroll
+    for (int h = 0; h < HC; h++) {
+      m[h] = -INFINITY;
+      l[h] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) q[h][i] = o[h][i] = 0.0f;
+      if (d < D) load8(reinterpret_cast<const T*>(a.q) + (size_t)t * a.q_stride + (size_t)(h0 + h) * D + d, a.q_vec, q[h]);
+    }
+    constexpr int U = HC == 1 ? 4 : 2;                // keys a round
+    for (int key = first + warp * (32 / width) * U; key < last; key += walkers * U) {
+      // (the bound is the warp's: its lanes take the shuffles below together)
+      float k[U][8], v[U][8];
+      bool in[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int at = key + u * (32 / width) + lanes_of;
+        in[u] = at < last;
+#pragma unroll
+        for (int i = 0; i < 8; i++) k[u][i] = v[u][i] = 0.0f;
+        const int page = in[u] ? page_of(a, req, at) : -1;
+        if (page >= 0 && d < D) {
+          const size_t x = row_at(a, page, hk, at) + d;
+          load8(reinterpret_cast<const T*>(a.cache) + x, 1, k[u]);
+          load8(reinterpret_cast<const T*>(a.cache) + x + value_offset(a), 1, v[u]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HC; h++) {
+        float s[U], mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          s[u] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) s[u] = fmaf(q[h][i], k[u][i], s[u]);
+        }
+        for (int w = 1; w < width; w <<= 1)
+#pragma unroll
+          for (int u = 0; u < U; u++) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          s[u] = in[u] ? s[u] : -INFINITY;
+          mx = fmaxf(mx, s[u]);
+        }
+        mx *= c2;
+        if (mx > m[h]) {
+          const float f = exp2f(m[h] - mx);
+          m[h] = mx;
+          l[h] *= f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) o[h][i] *= f;
+        }
+        const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const float p = exp2f(fmaf(s[u], c2, -ref));
+          l[h] += p;
+#pragma unroll
+          for (int i = 0; i < 8; i++) o[h][i] = fmaf(p, v[u][i], o[h][i]);
+        }
+      }
+    }
+    const int walker = tid / width;
+#pragma unroll
+    for (int h = 0; h < HC; h++) {
+      float* to = part + (walker * HC + h) * (D + 2);
+      if (d < D)
+#pragma unroll
+        for (int i = 0; i < 8; i++) to[d + i] = o[h][i];
+      if (sub == 0) {
+        to[D] = m[h];
+        to[D + 1] = l[h];
+      }
+    }
+  }
+  __syncthreads();
+  // the block's walkers
+  for (int x = tid; x < HC * (D + 1); x += OT) {
+    const int h = x / (D + 1), d = x % (D + 1);       // (column D: the sum of weights)
+    const float* from = part + h * (D + 2);
+    const int step = HC * (D + 2);
+    float M = -INFINITY, sum = 0.0f;
+    for (int w = 0; w < walkers; w++) M = fmaxf(M, from[w * step + D]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    for (int w = 0; w < walkers; w++) sum = fmaf(exp2f(from[w * step + D] - ref), from[w * step + (d == D ? D + 1 : d)], sum);
+    mine[h * (D + 2) + (d == D ? D + 1 : d)] = sum;
+    if (d == D) mine[h * (D + 2) + D] = M;
+  }
+  if (shares > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // (of the start)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  if (share == 0) {
+    pdl_wait();                                       // the prefixes' parts are there
+    // where this token's rows lie in them
+    const Parts ps = parts_of(a, plan, g, hk);
+    const int n0 = (t - plan.t0[g]) * gq + h0 - hk * gq;          // row of the block's first head in its group and key head
+    for (int x = tid; x < HC * ps.most; x += OT) {
+      const int h = x / ps.most, j = x % ps.most;
+      const long long row = part_row(a, ps, n0 + h, j);
+      const float2 ml = row < 0 ? make_float2(-INFINITY, 0.0f) : a.part_ml[row];
+      // (-inf: nothing was seen and no sums were written; scores that are all NaN have weights, but no maximum)
+      weight[x] = ml.y == 0.0f ? -INFINITY : ml.x == -INFINITY ? NAN : ml.x;
+    }
+    __syncthreads();
+    for (int x = tid; x < HC * D; x += OT) {
+      const int h = x / D, d = x % D;
+      auto own = [&](int z, int i) {
+        const float* at = mine + h * (D + 2) + i;
+        if (shares == 1) return *at;
+        uint32_t there;
+        float v;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(z));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+        return v;
+      };
+      float M = -INFINITY;
+      for (int j = 0; j < ps.most; j++) M = fmaxf(M, weight[h * ps.most + j]);
+      for (int z = 0; z < shares; z++) M = fmaxf(M, own(z, D));
+      const float ref = M == -INFINITY ? 0.0f : M;
+      float sum = 0.0f, total = 0.0f;
+      for (int z = 0; z < shares; z++) {
+        const float f = exp2f(own(z, D) - ref);
+        sum = fmaf(f, own(z, d), sum);
+        total = fmaf(f, own(z, D + 1), total);
+      }
+      for (int j = 0; j < ps.most; j++) {
+        const float mj = weight[h * ps.most + j];
+        if (mj == -INFINITY) continue;
+        const long long row = part_row(a, ps, n0 + h, j);
+        const float f = exp2f(mj - ref);
+        sum = fmaf(f, a.part_o[row * D + d], sum);
+        total = fmaf(f, a.part_ml[row].y, total);
+      }
+      reinterpret_cast<T*>(a.out)[(size_t)t * a.o_stride + (size_t)(h0 + h) * D + d] =
+          from_f32<T>(total == 0.0f ? 0.0f : sum / total);
+    }
+  }
+  if (shares > 1) {                                   // (block 0 has read the others' shared memory)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+template <typename T, int NC>
+int launch_general(const Args& a, cudaStream_t stream) {
+  const size_t smem = (size_t)((GR + GK) * (a.D + 4) + GK * NC * 64 + GR * (GK + 4)) * 4;
+  const cudaError_t e = cudaFuncSetAttribute(prefix_general_kernel<T, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             ((GR + GK) * (NC * 64 + 4) + GK * NC * 64 + GR * (GK + 4)) * 4);
+  if (e != cudaSuccess) return (int)e;
+  return sglc_launch(prefix_general_kernel<T, NC>, dim3(a.n_blocks), dim3(GT), smem, stream, 1, true, a);
+}
+template <typename T>
+int run_general(const Args& a, cudaStream_t stream) {
+  switch ((a.D + 63) / 64) {
+    case 1: return launch_general<T, 1>(a, stream);
+    case 2: return launch_general<T, 2>(a, stream);
+    case 3: return launch_general<T, 3>(a, stream);
+    default: return launch_general<T, 4>(a, stream);
+  }
+}
+
+template <typename T, int HC>
+int launch_own(const Args& a, int shares, cudaStream_t stream) {
+  const int walkers = OT / a.lanes;
+  const size_t smem = (size_t)((walkers + 1) * HC * (a.D + 2) + HC * most_parts(a)) * 4;
+  const cudaError_t e = cudaFuncSetAttribute(prefix_own_kernel<T, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+  if (e != cudaSuccess) return (int)e;
+  return sglc_launch(prefix_own_kernel<T, HC>, dim3((unsigned)((long long)a.T * (a.H / HC)), 1, shares), dim3(OT), smem, stream,
+                     shares, true, a);
+}
+template <typename T>
+int run_own(const Args& a, int max_own, cudaStream_t stream) {
+  const int gq = a.H / a.Hkv, hc = gq % 4 == 0 ? 4 : gq % 2 == 0 ? 2 : 1;
+  // blocks of a (token, heads): while there are fewer than four a multiprocessor, and 64 keys or more are left for each
+  int shares = 1;
+  while (shares < 8 && (long long)a.T * (a.H / hc) * shares * 2 <= 4LL * a.sms && max_own >= 64 * shares * 2) shares *= 2;
+  if (hc == 4) return launch_own<T, 4>(a, shares, stream);
+  if (hc == 2) return launch_own<T, 2>(a, shares, stream);
+  return launch_own<T, 1>(a, shares, stream);
+}
+
+int multiprocessors() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return n;
+}
+
+// The launch's blocks, rows an item and slots of the workspace, from sizes alone.
+bool lay_out(Args* a) {
+  a->sms = multiprocessors();
+  if (a->sms <= 0) return false;
+  a->n_blocks = 2 * a->sms;
+  a->slot_rows = GENERAL_ROWS;
+  a->key_tile = GENERAL_KEYS;
+  const long long rows = (long long)a->T * (a->H / a->Hkv);
+  a->slots = a->n_blocks + a->Hkv * (rows / GENERAL_ROWS + a->G);
+  a->lanes = 1;
+  while (a->lanes * 8 < a->D) a->lanes *= 2;
+  return true;
+}
+bool sizes_ok(int T, int R, int G, int H, int Hkv, int D) {
+  return T >= 0 && R >= 0 && G >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0;
+}
+}  // namespace
+
+// Floats of workspace that sglc_attention_prefix needs, or -1: the sizes are not taken.
+SGLC_API long long sglc_attention_prefix_workspace(int T, int G, int H, int Hkv, int D, int dtype) {
+  if (!sizes_ok(T, 0, G, H, Hkv, D) || D % 8 || D > 256 || G > MAX_GROUPS) return -1;
+  Args a = {};
+  a.T = T; a.G = G; a.H = H; a.Hkv = Hkv; a.D = D;
+  if (!lay_out(&a)) return -1;
+  return a.slots * a.slot_rows * (D + 2);
+}
+
+// q, out [T][stride] and cache, one layer's pages [n_pages][2][Hkv][page_size][D], of one dtype; table [R][bt_stride],
+// bt_width entries a row; token_req, positions [T]; group_start [G + 1]: the first token of each group, ascending;
+// shared_len [G].  Tokens before group_start[0] and from group_start[G] on are left out.  max_own: about how many keys of
+// its own a token has (it only sizes the launch).  workspace: floats, 16-byte aligned.  err: gets 4 where an index is out of
+// range (a request, a page, a position beyond the table): what it names is not read.
+SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void* cache, const int* table, long long bt_stride,
+                                   int bt_width, int R, const int* token_req, const int* positions, const int* group_start,
+                                   const int* shared_len, int G, void* out, long long o_stride, int T, int H, int Hkv, int D,
+                                   int page_size, int n_pages, float scale, int max_own, float* workspace, long long ws_floats,
+                                   int dtype, int* err, cudaStream_t stream) {
+  if (!sizes_ok(T, R, G, H, Hkv, D) || page_size <= 0 || n_pages < 0 || bt_width < 0 || !(scale > 0.0f) ||
+      (dtype != SGLC_F32 && dtype != SGLC_BF16))
+    return SGLC_ERR_ARGUMENT;
+  if (D % 8 || D > 256 || G > MAX_GROUPS || (long long)T * H > 0x7fffffffLL || ((uintptr_t)cache & 15)) return SGLC_ERR_UNSUPPORTED;
+  if (T == 0 || G == 0) return SGLC_OK;
+  Args a = {};
+  a.q = q; a.q_stride = q_stride; a.cache = cache;
+  a.q_vec = ((uintptr_t)q & 15) == 0 && q_stride * (dtype == SGLC_F32 ? 4 : 2) % 16 == 0;
+  a.table = table; a.bt_stride = bt_stride; a.R = R;
+  a.token_req = token_req; a.positions = positions; a.group_start = group_start; a.shared_len = shared_len;
+  a.out = out; a.o_stride = o_stride;
+  a.T = T; a.G = G; a.H = H; a.Hkv = Hkv; a.D = D; a.page_size = page_size; a.n_pages = n_pages; a.scale = scale;
+  const long long room = (long long)bt_width * page_size;
+  a.last_position = (int)(room > 0x7ffffff0LL ? 0x7ffffff0LL : room) - 1;
+  a.err = err;
+  if (!lay_out(&a)) return SGLC_ERR_ARGUMENT;
+  if (a.slots * a.slot_rows * (D + 2) > ws_floats || ((uintptr_t)workspace & 15)) return SGLC_ERR_ARGUMENT;
+  a.part_o = workspace;
+  a.part_ml = reinterpret_cast<float2*>(workspace + a.slots * a.slot_rows * D);
+  const int code = dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
+  if (code) return code;
+  return dtype == SGLC_F32 ? run_own<float>(a, max_own, stream) : run_own<__nv_bfloat16>(a, max_own, stream);
+}

@@ -1,0 +1,230 @@
+// What the launches of attention over shared prefixes agree on: the plan of items and shares that each block makes from
+// the groups' lengths, where parts lie in the workspace, and access to the paged cache with every index checked.
+#pragma once
+#include "common.cuh"
+
+namespace prefix {
+constexpr int MAX_GROUPS = 256;
+constexpr int GENERAL_ROWS = 64, GENERAL_KEYS = 64;       // an item's rows, a tile's keys
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+  const void* q;
+  long long q_stride;
+  int q_vec;                              // rows of queries can be read 16 bytes at a time
+  const void* cache;                      // [n_pages][2][Hkv][page_size][D]
+  const int* table;
+  long long bt_stride;
+  const int *token_req, *positions, *group_start, *shared_len;
+  void* out;
+  long long o_stride;
+  int T, R, G, H, Hkv, D, page_size, n_pages;
+  int last_position;                      // the last one that a row of the table has room for
+  float scale;
+  int* err;
+  // the launch
+  int sms, n_blocks, slot_rows, key_tile, lanes;
+  long long slots;
+  float* part_o;                          // [slots][slot_rows][D]: sums, against a maximum
+  float2* part_ml;                        // [slots][slot_rows]: that maximum (times log2 e), sum of weights
+};
+
+// Per group: first token, keys of the prefix, rows a key head, and what lies before it: items and tiles.
+struct Plan {
+  int t0[MAX_GROUPS], keys[MAX_GROUPS], rows[MAX_GROUPS];
+  int items[MAX_GROUPS + 1];
+  long long tiles[MAX_GROUPS + 1];
+};
+
+__device__ __forceinline__ void flag_index(const Args& a) {
+  if (a.err) atomicOr(a.err, SGLC_FLAG_INDEX);
+}
+__device__ __forceinline__ int request_of(const Args& a, int t) {
+  const int r = a.token_req ? a.token_req[t] : t;
+  if (r >= 0 && r < a.R) return r;
+  flag_index(a);
+  return -1;
+}
+__device__ __forceinline__ int page_of(const Args& a, int req, int key) {
+  const int page = a.table[(size_t)req * a.bt_stride + (unsigned)key / (unsigned)a.page_size];
+  if (page >= 0 && page < a.n_pages) return page;
+  flag_index(a);
+  return -1;
+}
+__device__ __forceinline__ size_t row_at(const Args& a, int page, int hk, int key) {
+  return (((size_t)page * 2 * a.Hkv + hk) * a.page_size + (unsigned)key % (unsigned)a.page_size) * a.D;
+}
+__device__ __forceinline__ size_t value_offset(const Args& a) { return (size_t)a.Hkv * a.page_size * a.D; }
+// keys of a prefix of `keys` that token t sees
+__device__ __forceinline__ int visible(const Args& a, int t, int keys) { return min(keys, max(a.positions[t], -1) + 1); }
+
+__device__ __forceinline__ int item_rows(const Args& a, int) { return a.slot_rows; }
+
+// Every thread of the block calls it.
+__device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
+  const int gq = a.H / a.Hkv;
+  for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
+    const int t0 = min(max(a.group_start[g], 0), a.T), t1 = min(max(a.group_start[g + 1], t0), a.T);
+    int keys = t1 > t0 ? min(max(a.shared_len[g], 0), a.last_position + 1) : 0;
+    if (keys > 0 && request_of(a, t0) < 0) keys = 0;
+    p.t0[g] = t0;
+    p.keys[g] = keys;
+    p.rows[g] = (t1 - t0) * gq;
+    const int items = keys > 0 ? a.Hkv * ((p.rows[g] + item_rows(a, g) - 1) / item_rows(a, g)) : 0;
+    p.items[g + 1] = items;
+    p.tiles[g + 1] = (long long)items * ((keys + a.key_tile - 1) / a.key_tile);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {                 // sums over the groups before
+    int items = 0;
+    long long tiles = 0;
+    for (int g0 = 0; g0 < a.G; g0 += 32) {
+      const int g = g0 + threadIdx.x;
+      int x = g < a.G ? p.items[g + 1] : 0;
+      long long y = g < a.G ? p.tiles[g + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, x, o);
+        const long long v = __shfl_up_sync(0xffffffffu, y, o);
+        if ((int)threadIdx.x >= o) {
+          x += u;
+          y += v;
+        }
+      }
+      if (g < a.G) {
+        p.items[g + 1] = items + x;
+        p.tiles[g + 1] = tiles + y;
+      }
+      items += __shfl_sync(0xffffffffu, x, 31);
+      tiles += __shfl_sync(0xffffffffu, y, 31);
+    }
+    if (threadIdx.x == 0) p.items[0] = 0, p.tiles[0] = 0;
+  }
+  __syncthreads();
+}
+
+// All tiles, items one after the other, go to `blocks` blocks in equal shares: block b has the tiles from b * tiles / blocks
+// on.  No share is empty.
+__device__ __forceinline__ int blocks_used(const Args& a, long long tiles) { return (int)min((long long)a.n_blocks, tiles); }
+__device__ __forceinline__ int block_of(long long tile, int blocks, long long tiles) {
+  return (int)(((tile + 1) * blocks - 1) / tiles);
+}
+
+// A block's piece of an item.
+struct Segment {
+  int g, item, hk, row_tile;              // group; item counted over all groups; its key head and rows
+  int t0, n_rows, keys, req;              // the group's first token, rows a key head, prefix, and whose pages hold it
+  int tile, tiles;                        // tiles of keys: the first, how many
+  long long at, end;                      // the piece's first tile and the end of the block's share, counted over all items
+};
+__device__ __forceinline__ Segment segment_at(const Args& a, const Plan& p, long long at, long long end) {
+  Segment s;
+  s.at = at;
+  s.end = end;
+  s.tiles = 0;
+  if (at >= end) return s;
+  int lo = 0, hi = a.G;                   // the last group whose tiles begin at or before `at` (it has some)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.tiles[mid] <= at) lo = mid; else hi = mid;
+  }
+  s.g = lo;
+  s.t0 = p.t0[lo];
+  s.n_rows = p.rows[lo];
+  s.keys = p.keys[lo];
+  s.req = a.token_req ? a.token_req[s.t0] : s.t0;
+  const int kt = (s.keys + a.key_tile - 1) / a.key_tile, rt = (s.n_rows + item_rows(a, lo) - 1) / item_rows(a, lo);
+  const int n = (int)((at - p.tiles[lo]) / kt);
+  s.tile = (int)((at - p.tiles[lo]) % kt);
+  s.tiles = (int)min((long long)(kt - s.tile), end - at);
+  s.item = p.items[lo] + n;
+  s.hk = n / rt;
+  s.row_tile = n % rt;
+  return s;
+}
+__device__ __forceinline__ Segment first_segment(const Args& a, const Plan& p) {
+  const long long tiles = p.tiles[a.G];
+  const int blocks = blocks_used(a, tiles);
+  if ((int)blockIdx.x >= blocks) return segment_at(a, p, 0, 0);
+  return segment_at(a, p, tiles * blockIdx.x / blocks, tiles * (blockIdx.x + 1) / blocks);
+}
+__device__ __forceinline__ Segment next_segment(const Args& a, const Plan& p, const Segment& s) {
+  return segment_at(a, p, s.at + s.tiles, s.end);
+}
+
+// The parts of a group's rows of one key head.  The piece that block b finds of item i lies in slot b + i of the workspace:
+// along the shares either the block or the item goes up by one, so no two pieces meet in one slot.
+struct Parts {
+  int most;                               // parts of a row, at most
+  int first_item, rows_item;
+  int kt, blocks;
+  long long first_tile, tiles;
+};
+__device__ __forceinline__ Parts parts_of(const Args& a, const Plan& p, int g, int hk) {
+  Parts x;
+  x.tiles = p.tiles[a.G];
+  x.blocks = blocks_used(a, x.tiles);
+  x.rows_item = item_rows(a, g);
+  x.kt = (p.keys[g] + a.key_tile - 1) / a.key_tile;
+  const int rt = (p.rows[g] + x.rows_item - 1) / x.rows_item;
+  x.first_item = p.items[g] + hk * rt;
+  x.first_tile = p.tiles[g] + (long long)hk * rt * x.kt;
+  // an item of kt tiles meets at most this many shares of tiles / blocks
+  x.most = x.kt == 0 ? 0 : (int)min((long long)x.blocks, ((long long)x.kt * x.blocks + x.tiles - 1) / x.tiles + 1);
+  return x;
+}
+// The workspace's row of part j of row n, or -1: it has no such part.
+__device__ __forceinline__ long long part_row(const Args& a, const Parts& x, int n, int j) {
+  const int i = n / x.rows_item;
+  const long long begin = x.first_tile + (long long)i * x.kt;
+  const int b = block_of(begin, x.blocks, x.tiles) + j;
+  if (b > block_of(begin + x.kt - 1, x.blocks, x.tiles) || b + x.first_item + i >= a.slots) return -1;
+  return (long long)(b + x.first_item + i) * a.slot_rows + n % x.rows_item;
+}
+// (room for the weights of a row's parts)
+static inline int most_parts(const Args& a) { return a.n_blocks + 1; }
+
+__device__ __forceinline__ int group_of(const Args& a, const Plan& p, int t) {
+  if (t < a.group_start[0] || t >= a.group_start[a.G]) return -1;
+  int lo = 0, hi = a.G;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.t0[mid] <= t) lo = mid; else hi = mid;
+  }
+  if (t - p.t0[lo] < p.rows[lo] / (a.H / a.Hkv)) return lo;
+  flag_index(a);                          // (starts that do not ascend)
+  return -1;
+}
+// Whether a piece has a slot.  It has, unless the groups' starts do not ascend and their tokens overlap.
+__device__ __forceinline__ bool slot_ok(const Args& a, const Segment& s) {
+  if (blockIdx.x + (long long)s.item < a.slots) return true;
+  flag_index(a);
+  return false;
+}
+
+// eight entries of a row; vec: it begins on 16 bytes
+__device__ __forceinline__ void load8(const float* p, int vec, float (&v)[8]) {
+  if (vec) {
+    const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = p[i];
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int vec, float (&v)[8]) {
+  if (vec) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __bfloat162float(p[i]);
+  }
+}
+}  // namespace prefix

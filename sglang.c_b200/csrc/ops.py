@@ -316,6 +316,59 @@ def kv_write(k_src, v_src, cache, slots, n_kv_heads, head_dim):
     _check(lib, code, "kv_write")
 
 
+def _on_current_device(what, *tensors):
+    """The kernels run on the current device's stream: every tensor has to lie there."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{here}")
+
+
+STEP_TABLES_REQUESTS = 16384     # requests step_tables takes (step_tables.cu: MAX_REQUESTS)
+
+
+def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_start, new_len, token_req, positions, slots,
+                left, status):
+    """A step's arrays made on the device, from lengths that lie there.  Request r of R holds kv_len[r] positions, whose
+    pages are in its row of block_table ([R, width], row stride free), and brings q_len[r] tokens (none: 0).  The pages
+    it needs for them are taken from free_pages, a stack whose first n_free[0] words are free pages, the top last
+    (as cache.pages.PagePool hands them out), and entered into its row.  Written: q_start [R+1], new_len [R] (lengths
+    after the step), token_req, positions and slots of all tokens, in the order of the requests, left[0] (pages that
+    stay free) and status[0].  What the arrays hold behind the last token stays as it was.
+
+    All or nothing: where the pages are too few (status 1), a row too short (2), the tokens more than the arrays hold (4)
+    or a length is out of range (8; sums of these), only status is written.  All arrays int32.  new_len and left are
+    not kv_len and n_free (every block reads those)."""
+    arrays = dict(q_len=q_len, kv_len=kv_len, free_pages=free_pages, n_free=n_free, q_start=q_start, new_len=new_len,
+                  token_req=token_req, positions=positions, slots=slots, left=left, status=status)
+    _need_cuda(block_table, *arrays.values())
+    _on_current_device("step_tables", block_table, *arrays.values())
+    for nm, t in arrays.items():
+        _i32(t, f"step_tables: {nm}")
+    R = q_len.numel()
+    if R > STEP_TABLES_REQUESTS:
+        raise KernelError(f"step_tables: {R} requests; at most {STEP_TABLES_REQUESTS}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < R \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1) or block_table.stride(0) < block_table.shape[1]:
+        raise KernelError(f"step_tables: block_table must be int32 rows for {R} requests")
+    T = token_req.numel()
+    if kv_len.numel() < R or new_len.numel() < R or q_start.numel() < R + 1 or positions.numel() != T or slots.numel() != T:
+        raise KernelError("step_tables: kv_len and new_len have an entry a request, q_start one more, and token_req, positions "
+                          "and slots one length")
+    if n_free.numel() < 1 or left.numel() < 1 or status.numel() < 1:
+        raise KernelError("step_tables: n_free, left and status are one word each")
+    if int(page_size) != page_size or not 0 < page_size <= 1 << 20:
+        raise KernelError(f"step_tables: page size {page_size}")
+    if left.data_ptr() == n_free.data_ptr() or (R and new_len.data_ptr() == kv_len.data_ptr()):
+        raise KernelError("step_tables: new_len and left must be other memory than kv_len and n_free")
+    lib = build.load("step_tables")
+    code = lib.sglc_step_tables(_ptr(q_len), _ptr(kv_len), _ptr(free_pages), free_pages.numel(), _ptr(n_free),
+                                _ptr(block_table), ctypes.c_longlong(block_table.stride(0)), block_table.shape[1], R,
+                                int(page_size), _ptr(q_start), _ptr(new_len), _ptr(token_req), _ptr(positions), _ptr(slots), T,
+                                _ptr(left), _ptr(status), _stream())
+    _check(lib, code, f"step_tables ({R} requests)")
+
+
 def _gate_args(gate, T, n_heads, width, what):
     """(pointer, row stride, 1 if per head) of an output gate: float32 rows of pre-activations, [T, n_heads]
     or [T, n_heads * width]; None: no gate."""
@@ -704,6 +757,78 @@ def attention_latent_decode(q, cache, block_table, token_req, positions, out, n_
     _check(lib, code, f"attention_latent_decode (dim {D}, up to {max_keys} keys)", n_kernels=2 if splits > 1 else 1)
 
 
+PREFIX_GROUPS = 256       # groups attention_prefix takes (attention_prefix.cuh: MAX_GROUPS)
+
+
+def attention_prefix_workspace(n_tokens, n_groups, n_heads, n_kv_heads, dim, dtype):
+    """float32 elements of workspace that attention_prefix takes for such a call on the current device."""
+    lib = build.load("attention_prefix")
+    lib.sglc_attention_prefix_workspace.restype = ctypes.c_longlong
+    if dtype not in _DT:
+        raise KernelError(f"attention_prefix: dtype {dtype} is not handled (float32 or bfloat16)")
+    n = lib.sglc_attention_prefix_workspace(int(n_tokens), int(n_groups), int(n_heads), int(n_kv_heads), int(dim), _DT[dtype])
+    if n < 0:
+        raise KernelError(f"attention_prefix: {n_heads} heads over {n_kv_heads} of size {dim}, {n_groups} groups: heads in whole "
+                          f"groups, sizes that are multiples of 8 up to 256, at most {PREFIX_GROUPS} groups of requests")
+    return n
+
+
+def attention_prefix(q, cache, block_table, token_req, positions, group_start, shared_len, out, n_heads, scale, max_own=256,
+                     workspace=None):
+    """Causal attention of a step's tokens over the paged cache [n_pages, 2, n_kv_heads, page_size, head_dim] (float32 or
+    bfloat16, as q and out), where requests share long prefixes: group g has the tokens group_start[g] ..
+    group_start[g+1]-1 (int32 [G+1], ascending), whose requests hold the same keys and values at positions
+    0..shared_len[g]-1 (int32 [G]; 0: none).  These are read once for all tokens of the group, through the row of
+    block_table ([R, width], row stride free) of its first token's request; the keys behind them through each token's
+    own row.  Token t belongs to request token_req[t] (None: to the t-th) and sees the keys of positions 0..positions[t]
+    (so one that lies inside the prefix sees its part of it; a position below 0 sees nothing and gives zeros).  A request
+    may bring any number of tokens; their keys and values are in the cache.  Tokens before group_start[0] or from
+    group_start[G] on are left out: their rows of out stay as they were.
+
+    q, out: [T, n_heads*head_dim] views, row stride free.  max_own: about how many keys of its own a token has, which only
+    sizes the launch.  workspace: float32, attention_prefix_workspace() elements or more, used by this call alone
+    until it is done (None: taken from torch's allocator).  An index out of range (a request, a page, a position beyond the
+    table's row) is not followed and sets the error word (tc_error_flag)."""
+    _need_cuda(q, cache, block_table, token_req, positions, group_start, shared_len, out, workspace)
+    _on_current_device("attention_prefix", q, cache, block_table, token_req, positions, group_start, shared_len, out, workspace)
+    for t, nm in ((token_req, "token_req"), (positions, "positions"), (group_start, "group_start"), (shared_len, "shared_len")):
+        if t is not None:
+            _i32(t, f"attention_prefix: {nm}")
+    if cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
+        raise KernelError("attention_prefix: the cache is [n_pages, 2, n_kv_heads, page_size, head_dim], contiguous")
+    n_pages, _, Hkv, page_size, D = cache.shape
+    T, G = q.shape[0], shared_len.numel()
+    if q.dim() != 2 or out.dim() != 2 or q.shape[1] != n_heads * D or out.shape[1] != n_heads * D or out.shape[0] < T \
+            or q.stride(1) != 1 or out.stride(1) != 1:
+        raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
+    if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise KernelError("attention_prefix: rows of out overlap")
+    if q.dtype != cache.dtype or out.dtype != cache.dtype:
+        raise KernelError("attention_prefix: queries, cache and output must have one dtype")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise KernelError("attention_prefix: block_table must be int32 rows")
+    if positions.numel() < T or (token_req is not None and token_req.numel() < T) or group_start.numel() != G + 1:
+        raise KernelError("attention_prefix: positions and token_req have an entry a token, group_start one more than shared_len")
+    if not (0.0 < scale < float("inf")):
+        raise KernelError(f"attention_prefix: scale {scale} must be positive")
+    if cache.data_ptr() % 16:
+        raise KernelError("attention_prefix: the cache must begin on 16 bytes")
+    need = attention_prefix_workspace(T, G, n_heads, Hkv, D, cache.dtype)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.float32, device=q.device)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.numel() < need \
+            or workspace.data_ptr() % 16:
+        raise KernelError(f"attention_prefix: the workspace must be {need} float32 elements or more, contiguous, on 16 bytes")
+    lib = build.load("attention_prefix")
+    code = lib.sglc_attention_prefix(
+        _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(cache), _ptr(block_table), ctypes.c_longlong(block_table.stride(0)),
+        block_table.shape[1], block_table.shape[0], _ptr(token_req), _ptr(positions), _ptr(group_start), _ptr(shared_len), G,
+        _ptr(out), ctypes.c_longlong(out.stride(0)), T, n_heads, Hkv, D, page_size, n_pages, ctypes.c_float(scale),
+        max(0, int(max_own)), _ptr(workspace), ctypes.c_longlong(workspace.numel()), _dt(q, "attention_prefix"),
+        _ptr(tc_error_flag(q.device)), _stream())
+    _check(lib, code, f"attention_prefix (head_dim {D})", n_kernels=2)
+
+
 # ---------------------------------------------------------------------------
 def attention_prefill_tc_supported(q, cache, scale):
     D = cache.shape[-1]
@@ -772,6 +897,49 @@ def sample(logits, params, hist_tok, hist_cnt, out_tok, out_logprob=None):
     code = lib.sglc_sample(_ptr(logits), logits.stride(0), V, n, _ptr(params), _ptr(hist_tok),
                            _ptr(hist_cnt), _ptr(out_tok), _ptr(out_logprob), _stream())
     _check(lib, code, "sample")
+
+
+TOP_TOKENS = 64      # alternatives token_logprobs gives a row (token_logprobs.cu: MAX_TOP)
+
+
+def token_logprobs(logits, tokens, logprob, entropy=None, place=None, top_ids=None, top_logprobs=None):
+    """Of every row of logits ([n, V] float32 or bfloat16, row stride free) the log-probability of tokens[row] (int32)
+    into logprob [n], and where they are given: entropy [n] of the row's distribution; place [n] (int32) of the token in the
+    order of choice (larger logits first, then smaller ids), counted from 0; the first k tokens of that order and
+    their log-probabilities, top_ids [n, k] (int32) and top_logprobs [n, k], k <= 64, row stride free.  float32 results.
+
+    A token outside 0..V-1 (say -1) asks for nothing: logprob 0, place -1.  tokens None: no row asks.  A logit
+    of -inf is a token that is not allowed; a row without any allowed one has log-probabilities -inf and entropy 0.  A
+    row with a logit that is NaN or +inf has NaN for both; in the order of choice NaN counts as -inf."""
+    _need_cuda(logits, tokens, logprob, entropy, place, top_ids, top_logprobs)
+    _on_current_device("token_logprobs", logits, tokens, logprob, entropy, place, top_ids, top_logprobs)
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError("token_logprobs: logits must be rows of a vocabulary")
+    n, V = logits.shape
+    for t, nm, dt in ((tokens, "tokens", torch.int32), (logprob, "logprob", torch.float32), (entropy, "entropy", torch.float32),
+                      (place, "place", torch.int32)):
+        if t is None and nm != "logprob":
+            continue
+        if t.dtype != dt or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+            raise KernelError(f"token_logprobs: {nm} must be a contiguous {dt} vector of an entry a row ({n})")
+    if (top_ids is None) != (top_logprobs is None):
+        raise KernelError("token_logprobs: top_ids and top_logprobs come together")
+    k = 0
+    if top_ids is not None:
+        k = top_ids.shape[1] if top_ids.dim() == 2 else -1
+        if k < 0 or tuple(top_ids.shape) != (n, k) or tuple(top_logprobs.shape) != (n, k) or top_ids.dtype != torch.int32 \
+                or top_logprobs.dtype != torch.float32:
+            raise KernelError("token_logprobs: top_ids must be int32 and top_logprobs float32, [rows, k] both")
+        if k > min(V, TOP_TOKENS):
+            raise KernelError(f"token_logprobs: {k} alternatives of {V} tokens; at most {TOP_TOKENS}")
+        if k > 1 and (top_ids.stride(1) != 1 or top_logprobs.stride(1) != 1) \
+                or n > 1 and k and top_ids.stride(0) != top_logprobs.stride(0):
+            raise KernelError("token_logprobs: top_ids and top_logprobs must be rows of one stride")
+    lib = build.load("token_logprobs")
+    code = lib.sglc_token_logprobs(_ptr(logits), ctypes.c_longlong(logits.stride(0)), _dt(logits, "token_logprobs"), n, V,
+                                   _ptr(tokens), _ptr(logprob), _ptr(entropy), _ptr(place), k, _ptr(top_ids), _ptr(top_logprobs),
+                                   ctypes.c_longlong(top_ids.stride(0) if k else 0), _stream())
+    _check(lib, code, f"token_logprobs (vocabulary {V})")
 
 
 # ---------------------------------------------------------------------------
