@@ -11,6 +11,7 @@
 // lengths.  What a block finds for (a piece of) an item goes to the workspace.  The second launch makes the tokens' own parts,
 // which it does while the first still runs, waits for that, and joins all parts of a (token, head).
 #include "attention_prefix.cuh"
+#include "attention_prefix_tc.cuh"
 
 SGLC_DEFINE_ERROR_STRING()
 
@@ -408,14 +409,15 @@ int multiprocessors() {
 }
 
 // The launch's blocks, rows an item and slots of the workspace, from sizes alone.
-bool lay_out(Args* a) {
+bool lay_out(Args* a, int dtype) {
   a->sms = multiprocessors();
   if (a->sms <= 0) return false;
-  a->n_blocks = 2 * a->sms;
-  a->slot_rows = GENERAL_ROWS;
-  a->key_tile = GENERAL_KEYS;
+  a->tc = dtype == SGLC_BF16 && (a->D == 64 || a->D == 128);
+  a->n_blocks = a->tc ? a->sms : 2 * a->sms;
+  a->slot_rows = a->tc ? TC_SLOT : GENERAL_ROWS;
+  a->key_tile = a->tc ? TC_KEYS : GENERAL_KEYS;
   const long long rows = (long long)a->T * (a->H / a->Hkv);
-  a->slots = a->n_blocks + a->Hkv * (rows / GENERAL_ROWS + a->G);
+  a->slots = a->n_blocks + a->Hkv * (rows / a->slot_rows + a->G);      // (items of 128 rows are the only ones of their group)
   a->lanes = 1;
   while (a->lanes * 8 < a->D) a->lanes *= 2;
   return true;
@@ -430,7 +432,7 @@ SGLC_API long long sglc_attention_prefix_workspace(int T, int G, int H, int Hkv,
   if (!sizes_ok(T, 0, G, H, Hkv, D) || D % 8 || D > 256 || G > MAX_GROUPS) return -1;
   Args a = {};
   a.T = T; a.G = G; a.H = H; a.Hkv = Hkv; a.D = D;
-  if (!lay_out(&a)) return -1;
+  if (!lay_out(&a, dtype)) return -1;
   return a.slots * a.slot_rows * (D + 2);
 }
 
@@ -459,11 +461,11 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   const long long room = (long long)bt_width * page_size;
   a.last_position = (int)(room > 0x7ffffff0LL ? 0x7ffffff0LL : room) - 1;
   a.err = err;
-  if (!lay_out(&a)) return SGLC_ERR_ARGUMENT;
+  if (!lay_out(&a, dtype)) return SGLC_ERR_ARGUMENT;
   if (a.slots * a.slot_rows * (D + 2) > ws_floats || ((uintptr_t)workspace & 15)) return SGLC_ERR_ARGUMENT;
   a.part_o = workspace;
   a.part_ml = reinterpret_cast<float2*>(workspace + a.slots * a.slot_rows * D);
-  const int code = dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
+  const int code = a.tc ? (D == 64 ? launch_tc<64, 11>(a, stream) : launch_tc<128, 4>(a, stream)) : dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
   if (code) return code;
   return dtype == SGLC_F32 ? run_own<float>(a, max_own, stream) : run_own<__nv_bfloat16>(a, max_own, stream);
 }

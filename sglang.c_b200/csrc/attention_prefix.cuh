@@ -24,6 +24,7 @@ struct Args {
   int* err;
   // the launch
   int sms, n_blocks, slot_rows, key_tile, lanes;
+  int tc;                                 // the tensor-core kernel
   long long slots;
   float* part_o;                          // [slots][slot_rows][D]: sums, against a maximum
   float2* part_ml;                        // [slots][slot_rows]: that maximum (times log2 e), sum of weights
@@ -58,7 +59,8 @@ __device__ __forceinline__ size_t value_offset(const Args& a) { return (size_t)a
 // keys of a prefix of `keys` that token t sees
 __device__ __forceinline__ int visible(const Args& a, int t, int keys) { return min(keys, max(a.positions[t], -1) + 1); }
 
-__device__ __forceinline__ int item_rows(const Args& a, int) { return a.slot_rows; }
+// Rows of an item of a group of so many rows a key head.
+__device__ __forceinline__ int rows_of_item(const Args& a, int rows) { return a.tc && rows <= 128 ? 128 : a.slot_rows; }
 
 // Every thread of the block calls it.
 __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
@@ -70,7 +72,8 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
     p.t0[g] = t0;
     p.keys[g] = keys;
     p.rows[g] = (t1 - t0) * gq;
-    const int items = keys > 0 ? a.Hkv * ((p.rows[g] + item_rows(a, g) - 1) / item_rows(a, g)) : 0;
+    const int per = rows_of_item(a, p.rows[g]);
+    const int items = keys > 0 ? a.Hkv * ((p.rows[g] + per - 1) / per) : 0;
     p.items[g + 1] = items;
     p.tiles[g + 1] = (long long)items * ((keys + a.key_tile - 1) / a.key_tile);
   }
@@ -113,6 +116,7 @@ __device__ __forceinline__ int block_of(long long tile, int blocks, long long ti
 // A block's piece of an item.
 struct Segment {
   int g, item, hk, row_tile;              // group; item counted over all groups; its key head and rows
+  int rows_item;                          // rows of an item of its group
   int t0, n_rows, keys, req;              // the group's first token, rows a key head, prefix, and whose pages hold it
   int tile, tiles;                        // tiles of keys: the first, how many
   long long at, end;                      // the piece's first tile and the end of the block's share, counted over all items
@@ -133,7 +137,8 @@ __device__ __forceinline__ Segment segment_at(const Args& a, const Plan& p, long
   s.n_rows = p.rows[lo];
   s.keys = p.keys[lo];
   s.req = a.token_req ? a.token_req[s.t0] : s.t0;
-  const int kt = (s.keys + a.key_tile - 1) / a.key_tile, rt = (s.n_rows + item_rows(a, lo) - 1) / item_rows(a, lo);
+  s.rows_item = rows_of_item(a, s.n_rows);
+  const int kt = (s.keys + a.key_tile - 1) / a.key_tile, rt = (s.n_rows + s.rows_item - 1) / s.rows_item;
   const int n = (int)((at - p.tiles[lo]) / kt);
   s.tile = (int)((at - p.tiles[lo]) % kt);
   s.tiles = (int)min((long long)(kt - s.tile), end - at);
@@ -156,6 +161,7 @@ __device__ __forceinline__ Segment next_segment(const Args& a, const Plan& p, co
 // along the shares either the block or the item goes up by one, so no two pieces meet in one slot.
 struct Parts {
   int most;                               // parts of a row, at most
+  int halves;                             // parts of a row in a slot: the tensor-core kernel's two groups of warps may share rows
   int first_item, rows_item;
   int kt, blocks;
   long long first_tile, tiles;
@@ -164,25 +170,26 @@ __device__ __forceinline__ Parts parts_of(const Args& a, const Plan& p, int g, i
   Parts x;
   x.tiles = p.tiles[a.G];
   x.blocks = blocks_used(a, x.tiles);
-  x.rows_item = item_rows(a, g);
+  x.rows_item = rows_of_item(a, p.rows[g]);
+  x.halves = a.tc && x.rows_item == 128 ? 2 : 1;
   x.kt = (p.keys[g] + a.key_tile - 1) / a.key_tile;
   const int rt = (p.rows[g] + x.rows_item - 1) / x.rows_item;
   x.first_item = p.items[g] + hk * rt;
   x.first_tile = p.tiles[g] + (long long)hk * rt * x.kt;
   // an item of kt tiles meets at most this many shares of tiles / blocks
-  x.most = x.kt == 0 ? 0 : (int)min((long long)x.blocks, ((long long)x.kt * x.blocks + x.tiles - 1) / x.tiles + 1);
+  x.most = x.kt == 0 ? 0 : x.halves * (int)min((long long)x.blocks, ((long long)x.kt * x.blocks + x.tiles - 1) / x.tiles + 1);
   return x;
 }
 // The workspace's row of part j of row n, or -1: it has no such part.
 __device__ __forceinline__ long long part_row(const Args& a, const Parts& x, int n, int j) {
   const int i = n / x.rows_item;
   const long long begin = x.first_tile + (long long)i * x.kt;
-  const int b = block_of(begin, x.blocks, x.tiles) + j;
+  const int half = x.halves == 2 ? j & 1 : 0, b = block_of(begin, x.blocks, x.tiles) + (x.halves == 2 ? j >> 1 : j);
   if (b > block_of(begin + x.kt - 1, x.blocks, x.tiles) || b + x.first_item + i >= a.slots) return -1;
-  return (long long)(b + x.first_item + i) * a.slot_rows + n % x.rows_item;
+  return (long long)(b + x.first_item + i) * a.slot_rows + half * 128 + n % x.rows_item;
 }
 // (room for the weights of a row's parts)
-static inline int most_parts(const Args& a) { return a.n_blocks + 1; }
+static inline int most_parts(const Args& a) { return (a.tc ? 2 : 1) * a.n_blocks; }
 
 __device__ __forceinline__ int group_of(const Args& a, const Plan& p, int t) {
   if (t < a.group_start[0] || t >= a.group_start[a.G]) return -1;

@@ -1,0 +1,416 @@
+// The prefixes' parts of attention over shared prefixes on the tensor cores: bfloat16, head sizes 64 and 128.
+//
+// One block per multiprocessor, a share of the tiles of 128 keys each (see the plan).  Scores S = Q K^T of 128 rows by 128 keys
+// go into tensor memory; a thread has a row of them, takes its maximum, turns them into bfloat16 weights
+// P = 2^(S c - m c) and puts these where the scores were, from where the second product O += P V takes them as its
+// first operand.  O stays in tensor memory and is scaled only where a row's maximum has grown by more than 2^8 (any
+// reference gives the same quotient; weights up to 2^8 lose no digits).  Two groups of four warps work in turn, so that one's
+// products run under the other's exponentials:
+//   rows of a group's key head <= 128: both groups have the same rows, and every other tile of keys each: what bounds it is
+//     the keys' way from memory, and a tile is met by 128 rows at most whatever is done;
+//   more: an item has 256 rows, 128 a group of warps, and each tile is met by both: half of the traffic for the same work.
+// Keys and values come page by page through the block table by TMA, in boxes of the largest power of two of rows that
+// divides the page, into a ring of tiles.  (No multicast.)
+#pragma once
+#include <string.h>
+
+#include "attention_prefix.cuh"
+#include "tc_common.cuh"
+
+namespace prefix {
+using namespace tc;
+
+constexpr int TC_KEYS = 128;             // keys a tile
+constexpr int TC_SLOT = 256;             // rows of a workspace slot
+constexpr int TC_WG = 128;               // threads (rows) of a group of warps
+constexpr int TC_THREADS = 2 * TC_WG + 64;     // warps 0-7 rows, warp 8 products and tensor memory, warp 9 loads
+constexpr int TC_MMA_WARP = 8, TC_LOAD_WARP = 9;
+constexpr int TC_TILE = TC_KEYS * 128;   // bytes of 128 rows by 64 columns
+constexpr int TC_MAX_UNITS = 11;
+
+struct TcCtl {
+  uint64_t full[TC_MAX_UNITS], empty[TC_MAX_UNITS];
+  uint64_t q_full, s_full[2], p_ready[2], o_full[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__device__ __forceinline__ void mma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :
+      : "r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y)),
+      "l"(reinterpret_cast<unsigned long long&>(z)));
+  return reinterpret_cast<float2&>(r);
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y)));
+  return reinterpret_cast<float2&>(r);
+}
+// byte offset of 16-byte piece c (0..7) of row r in a tile of rows of 128 bytes with the 128-byte swizzle
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// Tiles of a segment that group w of the warps works on, and its i-th.
+__device__ __forceinline__ int tiles_of(bool pair, int tiles, int w) { return pair ? tiles : (tiles + 1 - w) / 2; }
+__device__ __forceinline__ int tile_of(bool pair, int w, int i) { return pair ? i : 2 * i + w; }
+
+// UNITS: tiles of the ring; keys and values are a tile each.
+template <int D, int UNITS>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int box) {
+  constexpr int DB = D / 64, UNIT = DB * TC_TILE;
+  constexpr uint32_t TMEM_COLS = 512;               // scores (weights) 0..255, sums 256..256 + 2 D
+  // All shared memory is dynamic, so the tiles begin where the 128-byte swizzle needs them, on a multiple of 1024.
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;                               // two tiles of rows
+  uint8_t* ring = sQ + 2 * UNIT;
+  TcCtl& ctl = *reinterpret_cast<TcCtl*>(ring + UNITS * UNIT);
+  Plan& plan = *reinterpret_cast<Plan*>(ring + UNITS * UNIT + sizeof(TcCtl));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem) & 1023u) {                     // never seen; the tiles would be mis-swizzled
+    if (threadIdx.x == 0 && a.err) atomicOr(a.err, SGLC_FLAG_WAIT);
+    pdl_wait();
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < UNITS; i++) {
+      mbar_init(&ctl.full[i], 1);
+      mbar_init(&ctl.empty[i], 1);
+    }
+    mbar_init(&ctl.q_full, 2 * TC_WG);
+    for (int w = 0; w < 2; w++) {
+      mbar_init(&ctl.s_full[w], 1);
+      mbar_init(&ctl.p_ready[w], TC_WG);
+      mbar_init(&ctl.o_full[w], 1);
+    }
+    ctl.abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == TC_MMA_WARP) {
+    tmem_alloc(&ctl.tmem_base, TMEM_COLS);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_launch_dependents();                          // (not before: the second launch reads what came before this one)
+  make_plan(a, plan);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = ctl.tmem_base;
+  volatile int* abort_flag = &ctl.abort_flag;
+  const int gq = a.H / a.Hkv;
+
+  if (warp == TC_LOAD_WARP) {
+    // ---- loads: a lane a box; its page is asked for a tile ahead ----
+    Segment s = first_segment(a, plan), s2 = s;
+    int j = 0, j2 = 0;                              // s2, j2: the tile behind this one
+    auto box_row = [&](const Segment& x, int jj, int b) { return (x.tile + jj) * TC_KEYS + b * box; };
+    auto page_id = [&](const Segment& x, int jj, int b) {
+      const int key = box_row(x, jj, b);
+      if (x.tiles <= 0 || key >= x.keys || b * box >= TC_KEYS) return -1;
+      const int page = page_of(a, x.req, key);
+      return page < 0 ? a.n_pages : page;           // (a page outside reads as zeros)
+    };
+    int id_next = page_id(s, 0, lane);
+    uint32_t u = 0;
+    bool ok = true;
+    while (s.tiles > 0 && ok) {
+      const int id = id_next;
+      if (++j2 == s2.tiles) {
+        s2 = next_segment(a, plan, s2);
+        j2 = 0;
+      }
+      id_next = page_id(s2, j2, lane);
+      const int boxes = (min(TC_KEYS, s.keys - (s.tile + j) * TC_KEYS) + box - 1) / box;
+      for (int half = 0; half < 2 && ok; half++, u++) {
+        const int slot = u % UNITS;
+        if (u >= UNITS) {
+          int w = 1;
+          if (lane == 0) w = mbar_wait(&ctl.empty[slot], (u / UNITS - 1) & 1, abort_flag) ? 1 : 0;
+          ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+          if (!ok) break;
+        }
+        if (lane == 0) mbar_expect_tx(&ctl.full[slot], (uint32_t)boxes * DB * box * 128u);
+        __syncwarp();
+        for (int b = lane; b < boxes; b += 32) {
+          const int page = b < 32 ? id : page_id(s, j, b), in_page = box_row(s, j, b) % a.page_size;
+          for (int blk = 0; blk < DB; blk++)
+            tma_load_5d(ring + slot * UNIT + blk * TC_TILE + b * box * 128, &map_kv, &ctl.full[slot], blk * 64, in_page, s.hk, half,
+                        page);
+        }
+      }
+      s = s2;
+      j = j2;
+    }
+    if (!ok) {
+      // given up: what is still on its way into shared memory lands first (each unit's last load; a limit again)
+      for (uint32_t x = u > UNITS ? u - UNITS : 0; x < u; x++)
+        for (uint32_t i = 0; i < c_wait_limit && !mbar_try_wait(&ctl.full[x % UNITS], (x / UNITS) & 1); i++) {
+        }
+    }
+  } else if (warp == TC_MMA_WARP) {
+    // ---- products: lane 0 issues them ----
+    constexpr uint32_t idesc_s = idesc_bf16_f32(128, TC_KEYS, 0, 0);      // rows and keys both by columns of the head
+    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, 0, 1);            // values as they lie: keys by rows
+    uint32_t u0 = 0, q_turn = 0, p_turn[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      int w = 1;
+      if (lane == 0) w = mbar_wait(bar, parity, abort_flag) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+      return ok;
+    };
+    for (Segment s = first_segment(a, plan); s.tiles > 0 && ok; s = next_segment(a, plan, s)) {
+      const bool pair = s.rows_item == 2 * TC_WG;
+      if (!wait(&ctl.q_full, q_turn & 1)) break;
+      q_turn++;
+      auto scores = [&](int w, int i) {
+        const uint32_t u = u0 + 2 * tile_of(pair, w, i), slot = u % UNITS;
+        if (!wait(&ctl.full[slot], (u / UNITS) & 1)) return;
+        tc_fence_after_sync();
+        if (lane == 0) {
+          const uint32_t q0 = smem_u32(sQ + (pair ? w * UNIT : 0)), k0 = smem_u32(ring + slot * UNIT);
+#pragma unroll
+          for (int k = 0; k < D / 16; k++) {
+            const uint32_t off = (k / 4) * TC_TILE + (k % 4) * 32;
+            mma_bf16(tmem + w * 128, smem_desc_k_sw128(q0 + off), smem_desc_k_sw128(k0 + off), idesc_s, k > 0 ? 1u : 0u);
+          }
+          mma_commit(&ctl.s_full[w]);
+          if (!pair || w == 1) mma_commit(&ctl.empty[slot]);
+        }
+        __syncwarp();
+      };
+      const int n0 = tiles_of(pair, s.tiles, 0), n1 = tiles_of(pair, s.tiles, 1);
+      for (int w = 0; w < 2 && ok; w++)
+        if (w == 0 || n1 > 0) scores(w, 0);
+      for (int i = 0; i < n0 && ok; i++) {
+#pragma unroll 1
+        for (int w = 0; w < 2 && ok; w++) {
+          const int n = w ? n1 : n0;
+          if (i >= n) continue;
+          const int tile = tile_of(pair, w, i);
+          const uint32_t u = u0 + 2 * tile + 1, slot = u % UNITS;
+          if (!wait(&ctl.full[slot], (u / UNITS) & 1)) break;
+          // Behind the prefix's last key a tile holds what the page or the ring held, which may be no number: values there
+          // become zeros, as their weights are.
+          const int in_tile = s.keys - (s.tile + tile) * TC_KEYS;
+          if (in_tile < TC_KEYS && (!pair || w == 0)) {
+            for (int x = lane; x < (TC_KEYS - in_tile) * 8 * DB; x += 32) {
+              const int row = in_tile + x / (8 * DB), c = x % (8 * DB);
+              *reinterpret_cast<uint4*>(ring + slot * UNIT + (c / 8) * TC_TILE + row * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_proxy();
+            __syncwarp();
+          }
+          if (!wait(&ctl.p_ready[w], p_turn[w] & 1)) break;
+          p_turn[w]++;
+          tc_fence_after_sync();
+          if (lane == 0) {
+            const uint32_t v0 = smem_u32(ring + slot * UNIT);
+#pragma unroll
+            for (int k = 0; k < TC_KEYS / 16; k++)
+              mma_bf16_ta(tmem + 256 + w * D, tmem + w * 128 + 64 + k * 8, smem_desc_mn_sw128(v0 + k * 2048, TC_TILE, 1024), idesc_o,
+                          (i > 0 || k > 0) ? 1u : 0u);
+            if (!pair || w == 1) mma_commit(&ctl.empty[slot]);
+            if (i + 1 == n) mma_commit(&ctl.o_full[w]);
+          }
+          __syncwarp();
+          if (i + 1 < n) scores(w, i + 1);           // (they overwrite the weights that the product before them takes)
+        }
+      }
+      u0 += 2 * s.tiles;
+    }
+  } else {
+    // ---- rows: a thread a row; group w of four warps ----
+    const int w = warp >> 2, row = threadIdx.x & (TC_WG - 1);
+    const uint32_t tS = tmem + w * 128 + ((uint32_t)(warp & 3) << 21), tO = tmem + 256 + w * D + ((uint32_t)(warp & 3) << 21);
+    const float c2 = a.scale * LOG2E;
+    uint32_t s_turn = 0, o_turn = 0;
+    bool ok = true;
+    for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
+      const int rows_item = s.rows_item;
+      const bool pair = rows_item == 2 * TC_WG;
+      const int rows = min(rows_item, s.n_rows - s.row_tile * rows_item);      // of this item
+      const int mine = pair ? w * TC_WG + row : row;
+      const int n = s.row_tile * rows_item + mine, t = s.t0 + n / gq;
+      const bool valid = mine < rows;
+      const int lim = valid ? visible(a, t, s.keys) : 0;
+      // both groups are done with the item before (its products have been waited for): queries of this one
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      {
+        // (the same 128 rows for both groups: half of the columns each)
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)(s.hk * gq + n % gq) * D;
+        const int c0 = pair ? 0 : w * (D / 16), c1 = pair ? D / 8 : c0 + D / 16;
+        uint8_t* dst = sQ + (pair ? w * UNIT : 0);
+        for (int c = c0; c < c1; c++) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (valid) {
+            if (a.q_vec) {
+              x = *reinterpret_cast<const uint4*>(src + c * 8);
+            } else {
+              const unsigned short* h = reinterpret_cast<const unsigned short*>(src + c * 8);
+              x = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                             h[6] | (uint32_t)h[7] << 16);
+            }
+          }
+          *reinterpret_cast<uint4*>(dst + (c / 8) * TC_TILE + sw128(row, c % 8)) = x;
+        }
+      }
+      fence_async_proxy();
+      mbar_arrive(&ctl.q_full);
+      const bool busy = (warp & 3) * 32 + (pair ? w * TC_WG : 0) < rows;       // this warp has rows at all
+      const int tiles = tiles_of(pair, s.tiles, w);
+      float m = -INFINITY, l = 0.0f;
+      for (int i = 0; i < tiles && ok; i++) {
+        ok = mbar_wait(&ctl.s_full[w], s_turn & 1, abort_flag);
+        if (!ok) break;
+        s_turn++;
+        tc_fence_after_sync();
+        if (busy) {
+          // The scores of 64 keys at a time: the maximum over the first half, then over the second, which stays in registers and
+          // is turned into weights first; then the first half again.  (128 registers of scores would not leave room.)  The
+          // weights go over the second half of the scores.
+          const int in_tile = lim - (s.tile + tile_of(pair, w, i)) * TC_KEYS;  // keys of the tile that the row sees
+          const bool whole = __all_sync(0xffffffffu, in_tile >= TC_KEYS);
+          uint32_t v[2][32];
+          auto take = [&](int half) {
+            tmem_ld_32x32(tS + 64 * half, v[0]);
+            tmem_ld_32x32(tS + 64 * half + 32, v[1]);
+            tmem_ld_wait();
+            if (!whole) {
+#pragma unroll
+              for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int x = 0; x < 32; x++)
+                  if (64 * half + 32 * c + x >= in_tile) v[c][x] = 0xff800000u;       // -inf
+            }
+          };
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            take(half);
+#pragma unroll
+            for (int x = 0; x < 64; x++) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x >> 5][x & 31]));
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          float alpha = 1.0f;
+          if (m == -INFINITY) {
+            m = top;                                 // (a row's first keys: its sums are zero)
+          } else if ((top - m) * c2 > 8.0f) {
+            alpha = ex2_approx((m - top) * c2);
+            l *= alpha;
+            m = top;
+          }
+          const float neg = m == -INFINITY ? 0.0f : -m * c2;
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+          for (int half = 1; half >= 0; half--) {
+            if (half == 0) take(0);
+            uint32_t p[32];
+#pragma unroll
+            for (int x = 0; x < 32; x++) {
+              const uint32_t* y = &v[x / 16][2 * (x % 16)];
+              const float2 e = fma2(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), make_float2(c2, c2), make_float2(neg, neg));
+              const float2 pp = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+              sum[x & 1] = add2(sum[x & 1], pp);
+              const __nv_bfloat162 hh = __floats2bfloat162_rn(pp.x, pp.y);
+              p[x] = *reinterpret_cast<const uint32_t*>(&hh);
+            }
+            tmem_st_32x32(tS + 64 + 32 * half, p);
+          }
+          if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+            // (the product before these scores is done: they were issued behind it and have been waited for)
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(tO + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int x = 0; x < 32; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              tmem_st_32x32(tO + c, o);
+            }
+          }
+          sum[0] = add2(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
+          tmem_st_wait();
+        }
+        tc_fence_before_sync();
+        mbar_arrive(&ctl.p_ready[w]);
+      }
+      if (tiles > 0 && ok) {
+        ok = mbar_wait(&ctl.o_full[w], o_turn & 1, abort_flag);
+        o_turn++;
+        tc_fence_after_sync();
+      }
+      if (busy && ok) {
+        const long long at = (long long)(blockIdx.x + s.item) * TC_SLOT + (pair ? 0 : w * TC_WG) + mine;
+        const bool there = valid && slot_ok(a, s);
+        if (there) a.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * c2, l);
+        if (tiles > 0) {
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(tO + c, o);
+            tmem_ld_wait();
+            if (there)
+#pragma unroll
+              for (int x = 0; x < 32; x += 4)
+                *reinterpret_cast<float4*>(a.part_o + at * D + c + x) = make_float4(__uint_as_float(o[x]), __uint_as_float(o[x + 1]),
+                                                                                  __uint_as_float(o[x + 2]), __uint_as_float(o[x + 3]));
+          }
+        }
+      }
+      tc_fence_before_sync();
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && ctl.abort_flag && a.err) atomicOr(a.err, SGLC_FLAG_WAIT);
+  if (warp == TC_MMA_WARP) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// One layer's pages [n_pages][2][Hkv][page_size][D] as a 5-D tensor, in boxes of `box` rows of one page and head, 64 columns wide.
+static inline bool make_kv_map(CUtensorMap* out, const Args& a, int box) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t D = a.D, ps = a.page_size, Hkv = a.Hkv;
+  cuuint64_t dims[5] = {D, ps, Hkv, 2, (cuuint64_t)a.n_pages};
+  cuuint64_t strides[4] = {D * 2, ps * D * 2, Hkv * ps * D * 2, 2 * Hkv * ps * D * 2};
+  cuuint32_t boxes[5] = {64, (cuuint32_t)box, 1, 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(a.cache), dims, strides, boxes, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int UNITS>
+int launch_tc(const Args& a, cudaStream_t stream) {
+  static_assert(UNITS <= TC_MAX_UNITS, "the ring's barriers");
+  constexpr size_t smem = (size_t)(2 + UNITS) * (D / 64) * TC_TILE + sizeof(TcCtl) + sizeof(Plan);
+  static_assert(smem <= 227 * 1024, "shared memory of a block");
+  int box = 1;
+  while (box < TC_KEYS && a.page_size % (box * 2) == 0) box *= 2;
+  CUtensorMap map;
+  memset(&map, 0, sizeof(map));
+  if (!make_kv_map(&map, a, box)) return SGLC_ERR_UNSUPPORTED;
+  const cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D, UNITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  return sglc_launch(prefix_tc_kernel<D, UNITS>, dim3(a.n_blocks), dim3(TC_THREADS), smem, stream, 1, true, map, a, box);
+}
+}  // namespace prefix
