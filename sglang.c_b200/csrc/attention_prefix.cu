@@ -465,7 +465,7 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   if (a.slots * a.slot_rows * (D + 2) > ws_floats || ((uintptr_t)workspace & 15)) return SGLC_ERR_ARGUMENT;
   a.part_o = workspace;
   a.part_ml = reinterpret_cast<float2*>(workspace + a.slots * a.slot_rows * D);
-  const int code = a.tc ? (D == 64 ? launch_tc<64, 11>(a, stream) : launch_tc<128, 4>(a, stream)) : dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
+  const int code = a.tc ? (D == 64 ? launch_tc<64, 4>(a, stream) : launch_tc<128, 2>(a, stream)) : dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
   if (code) return code;
   return dtype == SGLC_F32 ? run_own<float>(a, max_own, stream) : run_own<__nv_bfloat16>(a, max_own, stream);
 }

@@ -21,16 +21,17 @@ namespace prefix {
 using namespace tc;
 
 constexpr int TC_KEYS = 128;             // keys a tile
+constexpr int TC_HALF = 64;              // keys a step: a group of warps has two buffers of scores
 constexpr int TC_SLOT = 256;             // rows of a workspace slot
 constexpr int TC_WG = 128;               // threads (rows) of a group of warps
-constexpr int TC_THREADS = 2 * TC_WG + 64;     // warps 0-7 rows, warp 8 products and tensor memory, warp 9 loads
-constexpr int TC_MMA_WARP = 8, TC_LOAD_WARP = 9;
+constexpr int TC_MMA_WARP = 8, TC_LOAD_WARP = 10;     // (warps 0-7 rows; 8 and 9 products; 10 loads keys, 11 values)
+constexpr int TC_THREADS = 384;
 constexpr int TC_TILE = TC_KEYS * 128;   // bytes of 128 rows by 64 columns
-constexpr int TC_MAX_UNITS = 11;
+constexpr int TC_MAX_RING = 4;
 
 struct TcCtl {
-  uint64_t full[TC_MAX_UNITS], empty[TC_MAX_UNITS];
-  uint64_t q_full, s_full[2], p_ready[2], o_full[2];
+  uint64_t full[2][TC_MAX_RING], empty[2][TC_MAX_RING];       // of keys, of values
+  uint64_t q_full, s_full[2][2], p_ready[2][2], o_done[2], o_full[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -67,18 +68,18 @@ __device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 
 __device__ __forceinline__ int tiles_of(bool pair, int tiles, int w) { return pair ? tiles : (tiles + 1 - w) / 2; }
 __device__ __forceinline__ int tile_of(bool pair, int w, int i) { return pair ? i : 2 * i + w; }
 
-// UNITS: tiles of the ring; keys and values are a tile each.
-template <int D, int UNITS>
+// RING: tiles of keys in shared memory, and as many of values.
+template <int D, int RING>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int box) {
   constexpr int DB = D / 64, UNIT = DB * TC_TILE;
-  constexpr uint32_t TMEM_COLS = 512;               // scores (weights) 0..255, sums 256..256 + 2 D
+  constexpr uint32_t TMEM_COLS = 512;               // scores and weights: 64 columns a buffer, 0..255; sums 256..256 + 2 D
   // All shared memory is dynamic, so the tiles begin where the 128-byte swizzle needs them, on a multiple of 1024.
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                               // two tiles of rows
-  uint8_t* ring = sQ + 2 * UNIT;
-  TcCtl& ctl = *reinterpret_cast<TcCtl*>(ring + UNITS * UNIT);
-  Plan& plan = *reinterpret_cast<Plan*>(ring + UNITS * UNIT + sizeof(TcCtl));
+  uint8_t* ring = sQ + 2 * UNIT;                    // RING tiles of keys, RING of values
+  TcCtl& ctl = *reinterpret_cast<TcCtl*>(ring + 2 * RING * UNIT);
+  Plan& plan = *reinterpret_cast<Plan*>(ring + 2 * RING * UNIT + sizeof(TcCtl));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023u) {                     // never seen; the tiles would be mis-swizzled
     if (threadIdx.x == 0 && a.err) atomicOr(a.err, SGLC_FLAG_WAIT);
@@ -86,14 +87,18 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
     return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < UNITS; i++) {
-      mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], 1);
-    }
+    for (int h = 0; h < 2; h++)
+      for (int i = 0; i < RING; i++) {
+        mbar_init(&ctl.full[h][i], 1);
+        mbar_init(&ctl.empty[h][i], 2);
+      }
     mbar_init(&ctl.q_full, 2 * TC_WG);
     for (int w = 0; w < 2; w++) {
-      mbar_init(&ctl.s_full[w], 1);
-      mbar_init(&ctl.p_ready[w], TC_WG);
+      for (int b = 0; b < 2; b++) {
+        mbar_init(&ctl.s_full[w][b], 1);
+        mbar_init(&ctl.p_ready[w][b], TC_WG);
+      }
+      mbar_init(&ctl.o_done[w], 1);                 // (every product's end; o_full: the last one of an item's piece)
       mbar_init(&ctl.o_full[w], 1);
     }
     ctl.abort_flag = 0;
@@ -113,139 +118,123 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
   volatile int* abort_flag = &ctl.abort_flag;
   const int gq = a.H / a.Hkv;
 
-  if (warp == TC_LOAD_WARP) {
-    // ---- loads: a lane a box; its page is asked for a tile ahead ----
-    Segment s = first_segment(a, plan), s2 = s;
-    int j = 0, j2 = 0;                              // s2, j2: the tile behind this one
-    auto box_row = [&](const Segment& x, int jj, int b) { return (x.tile + jj) * TC_KEYS + b * box; };
+  if (warp >= TC_LOAD_WARP) {
+    // ---- loads, a warp for keys and one for values: a lane a box, whose page is asked for a tile ahead ----
+    // (a copy takes a warp's turn for 200 cycles, whoever issues it: 16 pages of 16 rows a tile were 3,250 cycles in one warp)
+    const int half = warp - TC_LOAD_WARP;
+    uint8_t* mine = ring + half * RING * UNIT;
+    Segment s = first_segment(a, plan);
+    int j = 0;
     auto page_id = [&](const Segment& x, int jj, int b) {
-      const int key = box_row(x, jj, b);
-      if (x.tiles <= 0 || key >= x.keys || b * box >= TC_KEYS) return -1;
+      const int key = (x.tile + jj) * TC_KEYS + b * box;
+      if (x.tiles <= 0 || b * box >= TC_KEYS || key >= x.keys) return -1;
       const int page = page_of(a, x.req, key);
       return page < 0 ? a.n_pages : page;           // (a page outside reads as zeros)
     };
     int id_next = page_id(s, 0, lane);
     uint32_t u = 0;
     bool ok = true;
-    while (s.tiles > 0 && ok) {
-      const int id = id_next;
-      if (++j2 == s2.tiles) {
-        s2 = next_segment(a, plan, s2);
-        j2 = 0;
+    for (; s.tiles > 0; u++) {
+      const int id = id_next, slot = u % RING;
+      const int key0 = (s.tile + j) * TC_KEYS, boxes = (min(TC_KEYS, s.keys - key0) + box - 1) / box;
+      if (u >= RING) {
+        int w = 1;
+        if (lane == 0) w = mbar_wait(&ctl.empty[half][slot], (u / RING - 1) & 1, abort_flag) ? 1 : 0;
+        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+        if (!ok) break;
       }
-      id_next = page_id(s2, j2, lane);
-      const int boxes = (min(TC_KEYS, s.keys - (s.tile + j) * TC_KEYS) + box - 1) / box;
-      for (int half = 0; half < 2 && ok; half++, u++) {
-        const int slot = u % UNITS;
-        if (u >= UNITS) {
-          int w = 1;
-          if (lane == 0) w = mbar_wait(&ctl.empty[slot], (u / UNITS - 1) & 1, abort_flag) ? 1 : 0;
-          ok = __shfl_sync(0xffffffffu, w, 0) != 0;
-          if (!ok) break;
-        }
-        if (lane == 0) mbar_expect_tx(&ctl.full[slot], (uint32_t)boxes * DB * box * 128u);
-        __syncwarp();
-        for (int b = lane; b < boxes; b += 32) {
-          const int page = b < 32 ? id : page_id(s, j, b), in_page = box_row(s, j, b) % a.page_size;
-          for (int blk = 0; blk < DB; blk++)
-            tma_load_5d(ring + slot * UNIT + blk * TC_TILE + b * box * 128, &map_kv, &ctl.full[slot], blk * 64, in_page, s.hk, half,
-                        page);
-        }
+      if (lane == 0) mbar_expect_tx(&ctl.full[half][slot], (uint32_t)boxes * DB * box * 128u);
+      __syncwarp();
+      for (int b = lane; b < boxes; b += 32) {
+        const int page = b < 32 ? id : page_id(s, j, b), in_page = (key0 + b * box) % a.page_size;
+        for (int blk = 0; blk < DB; blk++)
+          tma_load_5d(mine + slot * UNIT + blk * TC_TILE + b * box * 128, &map_kv, &ctl.full[half][slot], blk * 64, in_page, s.hk, half,
+                      page);
       }
-      s = s2;
-      j = j2;
+      if (++j == s.tiles) {
+        s = next_segment(a, plan, s);
+        j = 0;
+      }
+      id_next = page_id(s, j, lane);
     }
-    if (!ok) {
-      // given up: what is still on its way into shared memory lands first (each unit's last load; a limit again)
-      for (uint32_t x = u > UNITS ? u - UNITS : 0; x < u; x++)
-        for (uint32_t i = 0; i < c_wait_limit && !mbar_try_wait(&ctl.full[x % UNITS], (x / UNITS) & 1); i++) {
+    if (!ok)                                        // given up: what is still on its way here lands first (a limit again)
+      for (uint32_t z = u - RING; z < u; z++)
+        for (uint32_t i = 0; i < c_wait_limit && !mbar_try_wait(&ctl.full[half][z % RING], (z / RING) & 1); i++) {
         }
-    }
-  } else if (warp == TC_MMA_WARP) {
-    // ---- products: lane 0 issues them ----
-    constexpr uint32_t idesc_s = idesc_bf16_f32(128, TC_KEYS, 0, 0);      // rows and keys both by columns of the head
-    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, 0, 1);            // values as they lie: keys by rows
-    uint32_t u0 = 0, q_turn = 0, p_turn[2] = {0, 0};
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      int w = 1;
-      if (lane == 0) w = mbar_wait(bar, parity, abort_flag) ? 1 : 0;
-      ok = __shfl_sync(0xffffffffu, w, 0) != 0;
-      return ok;
-    };
-    for (Segment s = first_segment(a, plan); s.tiles > 0 && ok; s = next_segment(a, plan, s)) {
-      const bool pair = s.rows_item == 2 * TC_WG;
-      if (!wait(&ctl.q_full, q_turn & 1)) break;
-      q_turn++;
-      auto scores = [&](int w, int i) {
-        const uint32_t u = u0 + 2 * tile_of(pair, w, i), slot = u % UNITS;
-        if (!wait(&ctl.full[slot], (u / UNITS) & 1)) return;
-        tc_fence_after_sync();
-        if (lane == 0) {
-          const uint32_t q0 = smem_u32(sQ + (pair ? w * UNIT : 0)), k0 = smem_u32(ring + slot * UNIT);
+  } else if (warp >= TC_MMA_WARP) {
+    // ---- products: a warp a group of rows' warps, whose elected thread issues them (an elected one, so that descriptors stay
+    // in uniform registers: issued by lane 0 of the whole warp a product took 150 cycles; one thread for both groups was
+    // what the others waited for: a wait that has nothing to wait for takes it 200 cycles) ----
+    // Step i of a group is half i % 2 of its tile i / 2, in buffer i % 2.  The weights of step i go over its scores;
+    // behind the product that takes them come the scores of step i + 2, and those of i + 1 are there meanwhile.
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = idesc_bf16_f32(128, TC_HALF, 0, 0);    // rows and keys both by columns of the head
+      constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, 0, 1);          // values as they lie: keys by rows
+      const int w = warp - TC_MMA_WARP;
+      const uint32_t k_at = smem_u32(ring), v_at = k_at + RING * UNIT, tS = tmem + w * 128, tO = tmem + 256 + w * D;
+      uint32_t u0 = 0, q_turn = 0, turn = 0;
+      bool ok = true;
+      for (Segment s = first_segment(a, plan); s.tiles > 0 && ok; s = next_segment(a, plan, s)) {
+        const bool pair = s.rows_item == 2 * TC_WG;
+        const uint32_t q_at = smem_u32(sQ) + (pair ? w * UNIT : 0);
+        ok = mbar_wait(&ctl.q_full, q_turn & 1, abort_flag);
+        if (!ok) break;
+        q_turn++;
+        // a tile is given back when both groups have taken it: where it is this one's alone, by two arrivals
+        auto give_back = [&](uint64_t* bar) {
+          mma_commit(bar);
+          if (!pair) mma_commit(bar);
+        };
+        auto scores = [&](int i) {
+          const uint32_t u = u0 + tile_of(pair, w, i >> 1), slot = u % RING;
+          if ((i & 1) == 0) {
+            ok = mbar_wait(&ctl.full[0][slot], (u / RING) & 1, abort_flag);
+            if (!ok) return;
+            tc_fence_after_sync();
+          }
+          const uint32_t k0 = k_at + slot * UNIT + (i & 1) * (TC_HALF * 128);
 #pragma unroll
           for (int k = 0; k < D / 16; k++) {
             const uint32_t off = (k / 4) * TC_TILE + (k % 4) * 32;
-            mma_bf16(tmem + w * 128, smem_desc_k_sw128(q0 + off), smem_desc_k_sw128(k0 + off), idesc_s, k > 0 ? 1u : 0u);
+            mma_bf16(tS + (i & 1) * TC_HALF, smem_desc_k_sw128(q_at + off), smem_desc_k_sw128(k0 + off), idesc_s, k > 0 ? 1u : 0u);
           }
-          mma_commit(&ctl.s_full[w]);
-          if (!pair || w == 1) mma_commit(&ctl.empty[slot]);
-        }
-        __syncwarp();
-      };
-      const int n0 = tiles_of(pair, s.tiles, 0), n1 = tiles_of(pair, s.tiles, 1);
-      for (int w = 0; w < 2 && ok; w++)
-        if (w == 0 || n1 > 0) scores(w, 0);
-      for (int i = 0; i < n0 && ok; i++) {
-#pragma unroll 1
-        for (int w = 0; w < 2 && ok; w++) {
-          const int n = w ? n1 : n0;
-          if (i >= n) continue;
-          const int tile = tile_of(pair, w, i);
-          const uint32_t u = u0 + 2 * tile + 1, slot = u % UNITS;
-          if (!wait(&ctl.full[slot], (u / UNITS) & 1)) break;
-          // Behind the prefix's last key a tile holds what the page or the ring held, which may be no number: values there
-          // become zeros, as their weights are.
-          const int in_tile = s.keys - (s.tile + tile) * TC_KEYS;
-          if (in_tile < TC_KEYS && (!pair || w == 0)) {
-            for (int x = lane; x < (TC_KEYS - in_tile) * 8 * DB; x += 32) {
-              const int row = in_tile + x / (8 * DB), c = x % (8 * DB);
-              *reinterpret_cast<uint4*>(ring + slot * UNIT + (c / 8) * TC_TILE + row * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_async_proxy();
-            __syncwarp();
-          }
-          if (!wait(&ctl.p_ready[w], p_turn[w] & 1)) break;
-          p_turn[w]++;
+          mma_commit(&ctl.s_full[w][i & 1]);
+          if (i & 1) give_back(&ctl.empty[0][slot]);
+        };
+        const int n = 2 * tiles_of(pair, s.tiles, w);
+        for (int i = 0; i < 2 && n > 0 && ok; i++) scores(i);
+        for (int i = 0; i < n && ok; i++) {
+          const uint32_t u = u0 + tile_of(pair, w, i >> 1), slot = u % RING;
+          if ((i & 1) == 0) ok = mbar_wait(&ctl.full[1][slot], (u / RING) & 1, abort_flag);
+          if (ok) ok = mbar_wait(&ctl.p_ready[w][i & 1], (turn >> 1) & 1, abort_flag);
+          if (!ok) break;
+          turn++;
           tc_fence_after_sync();
-          if (lane == 0) {
-            const uint32_t v0 = smem_u32(ring + slot * UNIT);
+          const uint32_t v0 = v_at + slot * UNIT + (i & 1) * (TC_HALF * 128);
 #pragma unroll
-            for (int k = 0; k < TC_KEYS / 16; k++)
-              mma_bf16_ta(tmem + 256 + w * D, tmem + w * 128 + 64 + k * 8, smem_desc_mn_sw128(v0 + k * 2048, TC_TILE, 1024), idesc_o,
-                          (i > 0 || k > 0) ? 1u : 0u);
-            if (!pair || w == 1) mma_commit(&ctl.empty[slot]);
-            if (i + 1 == n) mma_commit(&ctl.o_full[w]);
-          }
-          __syncwarp();
-          if (i + 1 < n) scores(w, i + 1);           // (they overwrite the weights that the product before them takes)
+          for (int k = 0; k < TC_HALF / 16; k++)
+            mma_bf16_ta(tO, tS + (i & 1) * TC_HALF + k * 8, smem_desc_mn_sw128(v0 + k * 2048, TC_TILE, 1024), idesc_o,
+                        (i > 0 || k > 0) ? 1u : 0u);
+          mma_commit(&ctl.o_done[w]);
+          if (i & 1) give_back(&ctl.empty[1][slot]);
+          if (i + 1 == n) mma_commit(&ctl.o_full[w]);
+          if (i + 2 < n) scores(i + 2);
         }
+        u0 += s.tiles;
       }
-      u0 += 2 * s.tiles;
     }
   } else {
     // ---- rows: a thread a row; group w of four warps ----
     const int w = warp >> 2, row = threadIdx.x & (TC_WG - 1);
-    const uint32_t tS = tmem + w * 128 + ((uint32_t)(warp & 3) << 21), tO = tmem + 256 + w * D + ((uint32_t)(warp & 3) << 21);
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21, tS = tmem + w * 128 + lanes, tO = tmem + 256 + w * D + lanes;
     const float c2 = a.scale * LOG2E;
-    uint32_t s_turn = 0, o_turn = 0;
+    uint32_t turn = 0, u0 = 0, o_turn = 0;          // steps, tiles and pieces so far
     bool ok = true;
     for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
-      const int rows_item = s.rows_item;
-      const bool pair = rows_item == 2 * TC_WG;
-      const int rows = min(rows_item, s.n_rows - s.row_tile * rows_item);      // of this item
+      const bool pair = s.rows_item == 2 * TC_WG;
+      const int rows = min(s.rows_item, s.n_rows - s.row_tile * s.rows_item);  // of this item
       const int mine = pair ? w * TC_WG + row : row;
-      const int n = s.row_tile * rows_item + mine, t = s.t0 + n / gq;
+      const int n = s.row_tile * s.rows_item + mine, t = s.t0 + n / gq;
       const bool valid = mine < rows;
       const int lim = valid ? visible(a, t, s.keys) : 0;
       // both groups are done with the item before (its products have been waited for): queries of this one
@@ -272,39 +261,27 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       fence_async_proxy();
       mbar_arrive(&ctl.q_full);
       const bool busy = (warp & 3) * 32 + (pair ? w * TC_WG : 0) < rows;       // this warp has rows at all
-      const int tiles = tiles_of(pair, s.tiles, w);
+      const int steps = 2 * tiles_of(pair, s.tiles, w);
       float m = -INFINITY, l = 0.0f;
-      for (int i = 0; i < tiles && ok; i++) {
-        ok = mbar_wait(&ctl.s_full[w], s_turn & 1, abort_flag);
+      for (int i = 0; i < steps && ok; i++, turn++) {
+        ok = mbar_wait(&ctl.s_full[w][i & 1], (turn >> 1) & 1, abort_flag);
         if (!ok) break;
-        s_turn++;
         tc_fence_after_sync();
         if (busy) {
-          // The scores of 64 keys at a time: the maximum over the first half, then over the second, which stays in registers and
-          // is turned into weights first; then the first half again.  (128 registers of scores would not leave room.)  The
-          // weights go over the second half of the scores.
-          const int in_tile = lim - (s.tile + tile_of(pair, w, i)) * TC_KEYS;  // keys of the tile that the row sees
-          const bool whole = __all_sync(0xffffffffu, in_tile >= TC_KEYS);
+          const uint32_t at = tS + (i & 1) * TC_HALF;
           uint32_t v[2][32];
-          auto take = [&](int half) {
-            tmem_ld_32x32(tS + 64 * half, v[0]);
-            tmem_ld_32x32(tS + 64 * half + 32, v[1]);
-            tmem_ld_wait();
-            if (!whole) {
+          tmem_ld_32x32(at, v[0]);
+          tmem_ld_32x32(at + 32, v[1]);
+          tmem_ld_wait();
+          const int in_step = lim - (s.tile + tile_of(pair, w, i >> 1)) * TC_KEYS - (i & 1) * TC_HALF;    // keys of it the row sees
+          if (!__all_sync(0xffffffffu, in_step >= TC_HALF)) {
 #pragma unroll
-              for (int c = 0; c < 2; c++)
-#pragma unroll
-                for (int x = 0; x < 32; x++)
-                  if (64 * half + 32 * c + x >= in_tile) v[c][x] = 0xff800000u;       // -inf
-            }
-          };
+            for (int x = 0; x < TC_HALF; x++)
+              if (x >= in_step) v[x >> 5][x & 31] = 0xff800000u;              // -inf
+          }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            take(half);
-#pragma unroll
-            for (int x = 0; x < 64; x++) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x >> 5][x & 31]));
-          }
+          for (int x = 0; x < TC_HALF; x++) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x >> 5][x & 31]));
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           float alpha = 1.0f;
           if (m == -INFINITY) {
@@ -314,27 +291,13 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
             l *= alpha;
             m = top;
           }
-          const float neg = m == -INFINITY ? 0.0f : -m * c2;
-          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-          for (int half = 1; half >= 0; half--) {
-            if (half == 0) take(0);
-            uint32_t p[32];
-#pragma unroll
-            for (int x = 0; x < 32; x++) {
-              const uint32_t* y = &v[x / 16][2 * (x % 16)];
-              const float2 e = fma2(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), make_float2(c2, c2), make_float2(neg, neg));
-              const float2 pp = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-              sum[x & 1] = add2(sum[x & 1], pp);
-              const __nv_bfloat162 hh = __floats2bfloat162_rn(pp.x, pp.y);
-              p[x] = *reinterpret_cast<const uint32_t*>(&hh);
-            }
-            tmem_st_32x32(tS + 64 + 32 * half, p);
-          }
           if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-            // (the product before these scores is done: they were issued behind it and have been waited for)
+            // The sums are scaled once the product before this step is done.  (The one before that is: this step's scores
+            // came behind it.)
+            ok = mbar_wait(&ctl.o_done[w], (turn - 1) & 1, abort_flag);
+            tc_fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = 0; ok && c < D; c += 32) {
               uint32_t o[32];
               tmem_ld_32x32(tO + c, o);
               tmem_ld_wait();
@@ -343,24 +306,51 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
               tmem_st_32x32(tO + c, o);
             }
           }
+          const float neg = m == -INFINITY ? 0.0f : -m * c2;
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          uint32_t p[32];
+#pragma unroll
+          for (int x = 0; x < 32; x++) {
+            const uint32_t* y = &v[x / 16][2 * (x % 16)];
+            const float2 e = fma2(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), make_float2(c2, c2), make_float2(neg, neg));
+            const float2 pp = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+            sum[x & 1] = add2(sum[x & 1], pp);
+            const __nv_bfloat162 hh = __floats2bfloat162_rn(pp.x, pp.y);
+            p[x] = *reinterpret_cast<const uint32_t*>(&hh);
+          }
+          tmem_st_32x32(at, p);
           sum[0] = add2(sum[0], sum[1]);
           l += sum[0].x + sum[0].y;
           tmem_st_wait();
         }
+        const int tile = tile_of(pair, w, i >> 1), in_tile = s.keys - (s.tile + tile) * TC_KEYS;
+        if (in_tile < TC_KEYS && (i & 1) == 0) {
+          // The end of the prefix: behind its last key a tile of values holds what the page or the ring held, which may be no
+          // number.  It becomes zeros, as the weights there are, before the weights are handed on.  (The tile that had this
+          // place in the ring before was this group's too, the ring being even, and behind a product that these scores came
+          // behind: so the parity tells this one's landing.  Where both groups take the tile both write the zeros.)
+          const uint32_t u = u0 + tile, slot = u % RING;
+          ok = mbar_wait(&ctl.full[1][slot], (u / RING) & 1, abort_flag);
+          if (!ok) break;
+          for (int x = row; x < (TC_KEYS - in_tile) * 8 * DB; x += TC_WG) {
+            const int r = in_tile + x / (8 * DB), c = x % (8 * DB);
+            *reinterpret_cast<uint4*>(ring + (RING + slot) * UNIT + (c / 8) * TC_TILE + r * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_proxy();
+        }
         tc_fence_before_sync();
-        mbar_arrive(&ctl.p_ready[w]);
+        mbar_arrive(&ctl.p_ready[w][i & 1]);
       }
-      if (tiles > 0 && ok) {
-        ok = mbar_wait(&ctl.o_full[w], o_turn & 1, abort_flag);
-        o_turn++;
+      if (steps > 0 && ok) {
+        ok = mbar_wait(&ctl.o_full[w], o_turn++ & 1, abort_flag);
         tc_fence_after_sync();
       }
       if (busy && ok) {
         const long long at = (long long)(blockIdx.x + s.item) * TC_SLOT + (pair ? 0 : w * TC_WG) + mine;
         const bool there = valid && slot_ok(a, s);
         if (there) a.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * c2, l);
-        if (tiles > 0) {
-#pragma unroll
+        if (steps > 0) {
+#pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32(tO + c, o);
@@ -374,6 +364,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
         }
       }
       tc_fence_before_sync();
+      u0 += s.tiles;
     }
   }
   tc_fence_before_sync();
@@ -399,18 +390,18 @@ static inline bool make_kv_map(CUtensorMap* out, const Args& a, int box) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int UNITS>
+template <int D, int RING>
 int launch_tc(const Args& a, cudaStream_t stream) {
-  static_assert(UNITS <= TC_MAX_UNITS, "the ring's barriers");
-  constexpr size_t smem = (size_t)(2 + UNITS) * (D / 64) * TC_TILE + sizeof(TcCtl) + sizeof(Plan);
+  static_assert(RING % 2 == 0 && RING <= TC_MAX_RING, "the ring's barriers");
+  constexpr size_t smem = (size_t)(2 + 2 * RING) * (D / 64) * TC_TILE + sizeof(TcCtl) + sizeof(Plan);
   static_assert(smem <= 227 * 1024, "shared memory of a block");
   int box = 1;
   while (box < TC_KEYS && a.page_size % (box * 2) == 0) box *= 2;
   CUtensorMap map;
   memset(&map, 0, sizeof(map));
   if (!make_kv_map(&map, a, box)) return SGLC_ERR_UNSUPPORTED;
-  const cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D, UNITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D, RING>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  return sglc_launch(prefix_tc_kernel<D, UNITS>, dim3(a.n_blocks), dim3(TC_THREADS), smem, stream, 1, true, map, a, box);
+  return sglc_launch(prefix_tc_kernel<D, RING>, dim3(a.n_blocks), dim3(TC_THREADS), smem, stream, 1, true, map, a, box);
 }
 }  // namespace prefix
