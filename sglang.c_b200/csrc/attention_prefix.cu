@@ -39,6 +39,7 @@ prefix_general_kernel(const Args a) {
   pdl_wait();
   pdl_launch_dependents();                // (here and not before: the second launch reads what came before this one)
   make_plan(a, plan);
+  record_groups(a, plan);
   const float c2 = a.scale * LOG2E;
   const int gq = a.H / a.Hkv;
   for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
@@ -165,6 +166,7 @@ prefix_general_kernel(const Args a) {
         }
       }
     }
+    if (tid == 0) record_item(a, s);
     const size_t slot = (size_t)(blockIdx.x + s.item) * a.slot_rows;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -184,126 +186,224 @@ prefix_general_kernel(const Args a) {
 }
 
 // ---- a token's own keys, and the parts joined ------------------------------------------------------------------------------
-// A block has HC query heads of one key head of one token, or a share of their keys (a cluster of up to 8 blocks).  A key's
-// row is spread over the lanes of a part of a warp, eight entries a lane; each such part walks keys of its own with a running
-// maximum of its own.
+// An item is HC query heads of one key head of one token.  A warp, or four, or a cluster of blocks of four take an item: a
+// row of keys lies over LW lanes of a warp, eight entries a lane, and each such part of a warp (a walker) walks keys of its
+// own with a running maximum of its own, then, once the first launch is done, parts of the prefix in the same way.  Walkers
+// meet by shuffles, warps in shared memory, blocks through the cluster's.  What bounds it: the keys' and the parts' way from
+// memory, and for few items the chain token -> request -> page -> key; so a lane of the warp holds a page's id each, and the
+// keys of a round are asked for together.
 constexpr int OT = 128;
 
-template <typename T, int HC>
+// Eight entries as they lie in memory.
+template <typename T> struct Raw;
+template <> struct Raw<__nv_bfloat16> {
+  uint4 x;
+  __device__ __forceinline__ void take(const __nv_bfloat16* p) { x = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { x = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Raw<float> {
+  float4 x, y;
+  __device__ __forceinline__ void take(const float* p) {
+    x = *reinterpret_cast<const float4*>(p);
+    y = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void zero() { x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  }
+};
+
+// A part of a softmax: maximum (times log2 e), sum of weights, and eight columns of the weighted sum.
+struct State {
+  float m, l, o[8];
+  __device__ __forceinline__ void join(float m2, float l2, const float (&o2)[8]) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top, f = exp2f(m - ref), f2 = exp2f(m2 - ref);
+    m = top;
+    l = l * f + l2 * f2;
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = o[i] * f + o2[i] * f2;
+  }
+};
+
+// LW: lanes of a row, or 0: a.lanes.  warps: 1 or 4 of an item.
+template <typename T, int HC, int LW>
 __global__ void __launch_bounds__(OT)
-prefix_own_kernel(const Args a) {
-  extern __shared__ __align__(16) float sm[];
-  __shared__ Plan plan;
-  const int D = a.D, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = a.H / a.Hkv;
+prefix_own_kernel(const Args a, int warps) {
+  extern __shared__ __align__(16) float sm[];          // [4 warps][HC][D + 2], for items of four warps
+  const int D = a.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = a.H / a.Hkv;
+  const int width = LW ? LW : a.lanes, of_warp = lane / width, sub = lane % width, per_warp = 32 / width;
   const int share = blockIdx.z, shares = gridDim.z;
-  const int chunks = a.H / HC, t = blockIdx.x / chunks, h0 = blockIdx.x % chunks * HC, hk = h0 / gq;
-  const int width = a.lanes, lanes_of = lane / width, sub = lane % width, walkers = OT / width;
-  float* part = sm;                                   // [walkers][HC][D + 2]: sums, then maximum and sum of weights
-  float* mine = part + walkers * HC * (D + 2);        // [HC][D + 2]: this block's
-  float* weight = mine + HC * (D + 2);                // [HC][prefix parts]
   if (shares > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_launch_dependents();
-  make_plan(a, plan);
-  const int g = group_of(a, plan, t);
-  if (g < 0) {                                        // a token behind or before all groups (the whole cluster leaves)
-    pdl_wait();
-    return;
+  const int chunks = a.H / HC;
+  const long long item = warps == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
+  const bool real = item < (long long)a.T * chunks;
+  const int t = real ? (int)(item / chunks) : 0, h0 = (int)(item - (long long)t * chunks) * HC, hk = real ? h0 / gq : 0;
+  // the token's group: the last one that begins at or before it
+  int g = -1;
+  for (int x = 0; real && x < a.G; x += 32) g += __popc(__ballot_sync(0xffffffffu, x + lane < a.G && a.group_start[x + lane] <= t));
+  int t0 = 0, t1 = 0;
+  if (g >= 0) group_tokens(a, g, t0, t1);
+  const bool inside = g >= 0 && t >= t0 && t < t1;
+  // (starts that do not ascend, with the token behind this group's end and before the last one's)
+  if (g >= 0 && !inside && t < a.group_start[a.G]) flag_index(a);
+  const int keys = inside ? prefix_keys(a, g, t0, t1) : 0, walker = warps == 1 ? of_warp : (share * 4 + warp) * per_warp + of_warp;
+  const int walkers = (warps == 1 ? 1 : 4 * shares) * per_warp, d = sub * 8;
+  const bool cols = d < D;
+  State st[HC];
+#pragma unroll
+  for (int h = 0; h < HC; h++) {
+    st[h].m = -INFINITY;
+    st[h].l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) st[h].o[i] = 0.0f;
   }
-  const float c2 = a.scale * LOG2E;
-  const int keys = plan.keys[g], pos = a.positions[t];
-  const int req = request_of(a, t);
-  const int n_all = min(pos, a.last_position) + 1, n_own = req < 0 ? 0 : max(0, n_all - keys);
-  if (pos > a.last_position && tid == 0 && share == 0) flag_index(a);
-  const int first = keys + (int)((long long)n_own * share / shares), last = keys + (int)((long long)n_own * (share + 1) / shares);
-  {
-    const int d = sub * 8;
-    float q[HC][8], m[HC], l[HC], o[HC][8];
+  if (inside) {
+    const float c2 = a.scale * LOG2E;
+    const int pos = a.positions[t], req = request_of(a, t);
+    if (pos > a.last_position) flag_index(a);
+    const int end = req < 0 ? keys : min(pos, a.last_position) + 1;          // own keys: keys .. end - 1
+    float q[HC][8];
 #pragma unroll
     for (int h = 0; h < HC; h++) {
-      m[h] = -INFINITY;
-      l[h] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; i++) q[h][i] = o[h][i] = 0.0f;
-      if (d < D) load8(reinterpret_cast<const T*>(a.q) + (size_t)t * a.q_stride + (size_t)(h0 + h) * D + d, a.q_vec, q[h]);
+      for (int i = 0; i < 8; i++) q[h][i] = 0.0f;
+      if (cols) load8(reinterpret_cast<const T*>(a.q) + (size_t)t * a.q_stride + (size_t)(h0 + h) * D + d, a.q_vec, q[h]);
     }
-    constexpr int U = HC == 1 ? 4 : 2;                // keys a round
-    for (int key = first + warp * (32 / width) * U; key < last; key += walkers * U) {
-      // (the bound is the warp's: its lanes take the shuffles below together)
-      float k[U][8], v[U][8];
-      bool in[U];
+    constexpr int U = sizeof(T) == 2 && HC < 4 ? 4 : 2;          // keys of a walker a round
+    const size_t v_at = value_offset(a);
+    // 32 pages at a time, a lane an id
+    for (int block0 = (unsigned)keys / (unsigned)a.page_size; (long long)block0 * a.page_size < end; block0 += 32) {
+      const long long stop = min((long long)end, (long long)(block0 + 32) * a.page_size);
+      const int first = max(keys, block0 * a.page_size), last = (int)stop;
+      const int id = (long long)(block0 + lane) * a.page_size < last ? page_of(a, req, (block0 + lane) * a.page_size) : -1;
+      for (int key0 = first + (walker - of_warp) * U; key0 < last; key0 += walkers * U) {
+        // (the bounds are the warp's: its lanes take the shuffles together)
+        Raw<T> k[U], v[U];
+        bool in[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int at = key + u * (32 / width) + lanes_of;
-        in[u] = at < last;
+        for (int u = 0; u < U; u++) {
+          const int key = key0 + u * per_warp + of_warp;
+          const int page = __shfl_sync(0xffffffffu, id, ((unsigned)key / (unsigned)a.page_size - block0) & 31);
+          in[u] = key < last;
+          k[u].zero();
+          v[u].zero();
+          if (in[u] && page >= 0 && cols) {
+            const T* x = reinterpret_cast<const T*>(a.cache) + row_at(a, page, hk, key) + d;
+            k[u].take(x);
+            v[u].take(x + v_at);
+          }
+        }
 #pragma unroll
-        for (int i = 0; i < 8; i++) k[u][i] = v[u][i] = 0.0f;
-        const int page = in[u] ? page_of(a, req, at) : -1;
-        if (page >= 0 && d < D) {
-          const size_t x = row_at(a, page, hk, at) + d;
-          load8(reinterpret_cast<const T*>(a.cache) + x, 1, k[u]);
-          load8(reinterpret_cast<const T*>(a.cache) + x + value_offset(a), 1, v[u]);
+        for (int h = 0; h < HC; h++) {
+          float s[U], mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            float x[8];
+            k[u].get(x);
+            s[u] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[u] = fmaf(q[h][i], x[i], s[u]);
+          }
+#pragma unroll
+          for (int w = 1; w < (LW ? LW : 32); w <<= 1) {
+            if (!LW && w >= width) break;
+#pragma unroll
+            for (int u = 0; u < U; u++) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+          }
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            s[u] = in[u] ? s[u] : -INFINITY;
+            mx = fmaxf(mx, s[u]);
+          }
+          mx *= c2;
+          if (mx > st[h].m) {
+            const float f = exp2f(st[h].m - mx);
+            st[h].m = mx;
+            st[h].l *= f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) st[h].o[i] *= f;
+          }
+          const float ref = st[h].m == -INFINITY ? 0.0f : st[h].m;
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            const float p = exp2f(fmaf(s[u], c2, -ref));
+            float x[8];
+            v[u].get(x);
+            st[h].l += p;
+#pragma unroll
+            for (int i = 0; i < 8; i++) st[h].o[i] = fmaf(p, x[i], st[h].o[i]);
+          }
         }
       }
+    }
+  }
+  pdl_wait();                                          // the prefixes' parts are there
+  if (keys > 0) {
+    const Parts ps = parts_of(a, g, t0, t1, hk, (t - t0) * gq + h0 - hk * gq);
+    for (int j = walker; j < ps.n; j += walkers) {
+      const long long at = part_row(a, ps, j);
+      if (at < 0) continue;
 #pragma unroll
       for (int h = 0; h < HC; h++) {
-        float s[U], mx = -INFINITY;
+        const float2 ml = a.part_ml[at + h];
+        if (ml.y == 0.0f) continue;                    // nothing was seen and no sums were written (NaN is not 0)
+        float o[8];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          s[u] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) s[u] = fmaf(q[h][i], k[u][i], s[u]);
-        }
-        for (int w = 1; w < width; w <<= 1)
-#pragma unroll
-          for (int u = 0; u < U; u++) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-          s[u] = in[u] ? s[u] : -INFINITY;
-          mx = fmaxf(mx, s[u]);
-        }
-        mx *= c2;
-        if (mx > m[h]) {
-          const float f = exp2f(m[h] - mx);
-          m[h] = mx;
-          l[h] *= f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) o[h][i] *= f;
-        }
-        const float ref = m[h] == -INFINITY ? 0.0f : m[h];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-          const float p = exp2f(fmaf(s[u], c2, -ref));
-          l[h] += p;
-#pragma unroll
-          for (int i = 0; i < 8; i++) o[h][i] = fmaf(p, v[u][i], o[h][i]);
-        }
-      }
-    }
-    const int walker = tid / width;
-#pragma unroll
-    for (int h = 0; h < HC; h++) {
-      float* to = part + (walker * HC + h) * (D + 2);
-      if (d < D)
-#pragma unroll
-        for (int i = 0; i < 8; i++) to[d + i] = o[h][i];
-      if (sub == 0) {
-        to[D] = m[h];
-        to[D + 1] = l[h];
+        for (int i = 0; i < 8; i++) o[i] = 0.0f;
+        if (cols) load8(a.part_o + (at + h) * D + d, 1, o);
+        st[h].join(ml.x, ml.y, o);
       }
     }
   }
-  __syncthreads();
-  // the block's walkers
-  for (int x = tid; x < HC * (D + 1); x += OT) {
-    const int h = x / (D + 1), d = x % (D + 1);       // (column D: the sum of weights)
-    const float* from = part + h * (D + 2);
-    const int step = HC * (D + 2);
-    float M = -INFINITY, sum = 0.0f;
-    for (int w = 0; w < walkers; w++) M = fmaxf(M, from[w * step + D]);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    for (int w = 0; w < walkers; w++) sum = fmaf(exp2f(from[w * step + D] - ref), from[w * step + (d == D ? D + 1 : d)], sum);
-    mine[h * (D + 2) + (d == D ? D + 1 : d)] = sum;
-    if (d == D) mine[h * (D + 2) + D] = M;
+  // the warp's walkers
+#pragma unroll
+  for (int h = 0; h < HC; h++)
+#pragma unroll
+    for (int w = 16; w >= (LW ? LW : 1); w >>= 1) {
+      if (!LW && w < width) break;
+      float o[8];
+      const float m = __shfl_xor_sync(0xffffffffu, st[h].m, w), l = __shfl_xor_sync(0xffffffffu, st[h].l, w);
+#pragma unroll
+      for (int i = 0; i < 8; i++) o[i] = __shfl_xor_sync(0xffffffffu, st[h].o[i], w);
+      st[h].join(m, l, o);
+    }
+  if (warps == 1) {
+    if (inside && of_warp == 0 && cols) {
+#pragma unroll
+      for (int h = 0; h < HC; h++) {
+        const float f = st[h].l == 0.0f ? 0.0f : 1.0f / st[h].l;
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = st[h].l == 0.0f ? 0.0f : st[h].o[i] * f;
+        store8(reinterpret_cast<T*>(a.out) + (size_t)t * a.o_stride + (size_t)(h0 + h) * D + d, a.o_vec, o);
+      }
+    }
+    return;
+  }
+  // the block's warps, and the cluster's blocks
+  const int one = HC * (D + 2);
+  if (of_warp == 0) {
+#pragma unroll
+    for (int h = 0; h < HC; h++) {
+      float* to = sm + warp * one + h * (D + 2);
+      if (cols)
+#pragma unroll
+        for (int i = 0; i < 8; i++) to[d + i] = st[h].o[i];
+      if (sub == 0) {
+        to[D] = st[h].m;
+        to[D + 1] = st[h].l;
+      }
+    }
   }
   if (shares > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // (of the start)
@@ -312,53 +412,29 @@ prefix_own_kernel(const Args a) {
   } else {
     __syncthreads();
   }
-  if (share == 0) {
-    pdl_wait();                                       // the prefixes' parts are there
-    // where this token's rows lie in them
-    const Parts ps = parts_of(a, plan, g, hk);
-    const int n0 = (t - plan.t0[g]) * gq + h0 - hk * gq;          // row of the block's first head in its group and key head
-    for (int x = tid; x < HC * ps.most; x += OT) {
-      const int h = x / ps.most, j = x % ps.most;
-      const long long row = part_row(a, ps, n0 + h, j);
-      const float2 ml = row < 0 ? make_float2(-INFINITY, 0.0f) : a.part_ml[row];
-      // (-inf: nothing was seen and no sums were written; scores that are all NaN have weights, but no maximum)
-      weight[x] = ml.y == 0.0f ? -INFINITY : ml.x == -INFINITY ? NAN : ml.x;
-    }
-    __syncthreads();
-    for (int x = tid; x < HC * D; x += OT) {
-      const int h = x / D, d = x % D;
-      auto own = [&](int z, int i) {
-        const float* at = mine + h * (D + 2) + i;
-        if (shares == 1) return *at;
-        uint32_t there;
-        float v;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(z));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-        return v;
-      };
-      float M = -INFINITY;
-      for (int j = 0; j < ps.most; j++) M = fmaxf(M, weight[h * ps.most + j]);
-      for (int z = 0; z < shares; z++) M = fmaxf(M, own(z, D));
+  if (share == 0 && inside) {
+    auto other = [&](int z, int i) {                   // word i of warp z of the cluster
+      if (z < 4) return sm[z * one + i];
+      uint32_t there;
+      float v;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(sm + (z & 3) * one + i)), "r"(z >> 2));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+      return v;
+    };
+    for (int x = threadIdx.x; x < HC * D; x += OT) {
+      const int h = x / D, c = x - h * D, at = h * (D + 2);
+      float M = -INFINITY, sum = 0.0f, total = 0.0f;
+      for (int z = 0; z < 4 * shares; z++) M = fmaxf(M, other(z, at + D));
       const float ref = M == -INFINITY ? 0.0f : M;
-      float sum = 0.0f, total = 0.0f;
-      for (int z = 0; z < shares; z++) {
-        const float f = exp2f(own(z, D) - ref);
-        sum = fmaf(f, own(z, d), sum);
-        total = fmaf(f, own(z, D + 1), total);
+      for (int z = 0; z < 4 * shares; z++) {
+        const float f = exp2f(other(z, at + D) - ref);
+        sum = fmaf(f, other(z, at + c), sum);
+        total = fmaf(f, other(z, at + D + 1), total);
       }
-      for (int j = 0; j < ps.most; j++) {
-        const float mj = weight[h * ps.most + j];
-        if (mj == -INFINITY) continue;
-        const long long row = part_row(a, ps, n0 + h, j);
-        const float f = exp2f(mj - ref);
-        sum = fmaf(f, a.part_o[row * D + d], sum);
-        total = fmaf(f, a.part_ml[row].y, total);
-      }
-      reinterpret_cast<T*>(a.out)[(size_t)t * a.o_stride + (size_t)(h0 + h) * D + d] =
-          from_f32<T>(total == 0.0f ? 0.0f : sum / total);
+      reinterpret_cast<T*>(a.out)[(size_t)t * a.o_stride + (size_t)(h0 + h) * D + c] = from_f32<T>(total == 0.0f ? 0.0f : sum / total);
     }
   }
-  if (shares > 1) {                                   // (block 0 has read the others' shared memory)
+  if (shares > 1) {                                    // (block 0 has read the others' shared memory)
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
@@ -382,24 +458,31 @@ int run_general(const Args& a, cudaStream_t stream) {
   }
 }
 
+template <typename T, int HC, int LW>
+int launch_own(const Args& a, int warps, int shares, cudaStream_t stream) {
+  const size_t smem = warps == 1 ? 0 : (size_t)4 * HC * (a.D + 2) * 4;
+  const long long items = (long long)a.T * (a.H / HC);
+  return sglc_launch(prefix_own_kernel<T, HC, LW>, dim3((unsigned)(warps == 1 ? (items + 3) / 4 : items), 1, shares), dim3(OT), smem,
+                     stream, shares, true, a, warps);
+}
 template <typename T, int HC>
-int launch_own(const Args& a, int shares, cudaStream_t stream) {
-  const int walkers = OT / a.lanes;
-  const size_t smem = (size_t)((walkers + 1) * HC * (a.D + 2) + HC * most_parts(a)) * 4;
-  const cudaError_t e = cudaFuncSetAttribute(prefix_own_kernel<T, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
-  if (e != cudaSuccess) return (int)e;
-  return sglc_launch(prefix_own_kernel<T, HC>, dim3((unsigned)((long long)a.T * (a.H / HC)), 1, shares), dim3(OT), smem, stream,
-                     shares, true, a);
+int choose_own(const Args& a, int warps, int shares, cudaStream_t stream) {
+  if (a.lanes == 8) return launch_own<T, HC, 8>(a, warps, shares, stream);
+  if (a.lanes == 16) return launch_own<T, HC, 16>(a, warps, shares, stream);
+  return launch_own<T, HC, 0>(a, warps, shares, stream);
 }
 template <typename T>
 int run_own(const Args& a, int max_own, cudaStream_t stream) {
   const int gq = a.H / a.Hkv, hc = gq % 4 == 0 ? 4 : gq % 2 == 0 ? 2 : 1;
-  // blocks of a (token, heads): while there are fewer than four a multiprocessor, and 64 keys or more are left for each
+  const long long items = (long long)a.T * (a.H / hc);
+  // A warp an item where the items fill the multiprocessors and their own keys are few; else four, and blocks of a
+  // cluster while there are fewer than four a multiprocessor and 64 keys or more are left for each.
+  const int warps = items >= 16LL * a.sms && max_own <= 128 ? 1 : 4;
   int shares = 1;
-  while (shares < 8 && (long long)a.T * (a.H / hc) * shares * 2 <= 4LL * a.sms && max_own >= 64 * shares * 2) shares *= 2;
-  if (hc == 4) return launch_own<T, 4>(a, shares, stream);
-  if (hc == 2) return launch_own<T, 2>(a, shares, stream);
-  return launch_own<T, 1>(a, shares, stream);
+  while (warps == 4 && shares < 8 && items * shares * 2 <= 4LL * a.sms && max_own >= 64 * shares * 2) shares *= 2;
+  if (hc == 4) return choose_own<T, 4>(a, warps, shares, stream);
+  if (hc == 2) return choose_own<T, 2>(a, warps, shares, stream);
+  return choose_own<T, 1>(a, warps, shares, stream);
 }
 
 int multiprocessors() {
@@ -422,6 +505,8 @@ bool lay_out(Args* a, int dtype) {
   while (a->lanes * 8 < a->D) a->lanes *= 2;
   return true;
 }
+// floats of workspace: the parts' sums, their (maximum, sum of weights), the groups' first items, the items' blocks
+long long words(const Args& a) { return a.slots * a.slot_rows * (a.D + 2) + (a.G + 1) / 2 * 2 + 2 * a.slots; }
 bool sizes_ok(int T, int R, int G, int H, int Hkv, int D) {
   return T >= 0 && R >= 0 && G >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0;
 }
@@ -433,7 +518,7 @@ SGLC_API long long sglc_attention_prefix_workspace(int T, int G, int H, int Hkv,
   Args a = {};
   a.T = T; a.G = G; a.H = H; a.Hkv = Hkv; a.D = D;
   if (!lay_out(&a, dtype)) return -1;
-  return a.slots * a.slot_rows * (D + 2);
+  return words(a);
 }
 
 // q, out [T][stride] and cache, one layer's pages [n_pages][2][Hkv][page_size][D], of one dtype; table [R][bt_stride],
@@ -462,9 +547,12 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   a.last_position = (int)(room > 0x7ffffff0LL ? 0x7ffffff0LL : room) - 1;
   a.err = err;
   if (!lay_out(&a, dtype)) return SGLC_ERR_ARGUMENT;
-  if (a.slots * a.slot_rows * (D + 2) > ws_floats || ((uintptr_t)workspace & 15)) return SGLC_ERR_ARGUMENT;
+  if (words(a) > ws_floats || ((uintptr_t)workspace & 15)) return SGLC_ERR_ARGUMENT;
   a.part_o = workspace;
   a.part_ml = reinterpret_cast<float2*>(workspace + a.slots * a.slot_rows * D);
+  a.first_item = reinterpret_cast<int*>(a.part_ml + a.slots * a.slot_rows);
+  a.item_blocks = reinterpret_cast<int2*>(a.first_item + (G + 1) / 2 * 2);
+  a.o_vec = ((uintptr_t)out & 15) == 0 && o_stride * (dtype == SGLC_F32 ? 4 : 2) % 16 == 0;
   const int code = a.tc ? (D == 64 ? launch_tc<64, 4>(a, stream) : launch_tc<128, 2>(a, stream)) : dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
   if (code) return code;
   return dtype == SGLC_F32 ? run_own<float>(a, max_own, stream) : run_own<__nv_bfloat16>(a, max_own, stream);

@@ -18,6 +18,7 @@ struct Args {
   const int *token_req, *positions, *group_start, *shared_len;
   void* out;
   long long o_stride;
+  int o_vec;                              // (so can rows of results)
   int T, R, G, H, Hkv, D, page_size, n_pages;
   int last_position;                      // the last one that a row of the table has room for
   float scale;
@@ -28,6 +29,8 @@ struct Args {
   long long slots;
   float* part_o;                          // [slots][slot_rows][D]: sums, against a maximum
   float2* part_ml;                        // [slots][slot_rows]: that maximum (times log2 e), sum of weights
+  int* first_item;                        // [G]: items of the groups before
+  int2* item_blocks;                      // [slots]: the first and the last block that has a piece of the item
 };
 
 // Per group: first token, keys of the prefix, rows a key head, and what lies before it: items and tiles.
@@ -59,6 +62,16 @@ __device__ __forceinline__ size_t value_offset(const Args& a) { return (size_t)a
 // keys of a prefix of `keys` that token t sees
 __device__ __forceinline__ int visible(const Args& a, int t, int keys) { return min(keys, max(a.positions[t], -1) + 1); }
 
+// A group's tokens and how many keys of its prefix there are.
+__device__ __forceinline__ void group_tokens(const Args& a, int g, int& t0, int& t1) {
+  t0 = min(max(a.group_start[g], 0), a.T);
+  t1 = min(max(a.group_start[g + 1], t0), a.T);
+}
+__device__ __forceinline__ int prefix_keys(const Args& a, int g, int t0, int t1) {
+  const int keys = t1 > t0 ? min(max(a.shared_len[g], 0), a.last_position + 1) : 0;
+  return keys > 0 && request_of(a, t0) < 0 ? 0 : keys;
+}
+
 // Rows of an item of a group of so many rows a key head.
 __device__ __forceinline__ int rows_of_item(const Args& a, int rows) { return a.tc && rows <= 128 ? 128 : a.slot_rows; }
 
@@ -66,9 +79,9 @@ __device__ __forceinline__ int rows_of_item(const Args& a, int rows) { return a.
 __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
   const int gq = a.H / a.Hkv;
   for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-    const int t0 = min(max(a.group_start[g], 0), a.T), t1 = min(max(a.group_start[g + 1], t0), a.T);
-    int keys = t1 > t0 ? min(max(a.shared_len[g], 0), a.last_position + 1) : 0;
-    if (keys > 0 && request_of(a, t0) < 0) keys = 0;
+    int t0, t1;
+    group_tokens(a, g, t0, t1);
+    const int keys = prefix_keys(a, g, t0, t1);
     p.t0[g] = t0;
     p.keys[g] = keys;
     p.rows[g] = (t1 - t0) * gq;
@@ -109,9 +122,6 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
 // All tiles, items one after the other, go to `blocks` blocks in equal shares: block b has the tiles from b * tiles / blocks
 // on.  No share is empty.
 __device__ __forceinline__ int blocks_used(const Args& a, long long tiles) { return (int)min((long long)a.n_blocks, tiles); }
-__device__ __forceinline__ int block_of(long long tile, int blocks, long long tiles) {
-  return (int)(((tile + 1) * blocks - 1) / tiles);
-}
 
 // A block's piece of an item.
 struct Segment {
@@ -157,56 +167,47 @@ __device__ __forceinline__ Segment next_segment(const Args& a, const Plan& p, co
   return segment_at(a, p, s.at + s.tiles, s.end);
 }
 
-// The parts of a group's rows of one key head.  The piece that block b finds of item i lies in slot b + i of the workspace:
-// along the shares either the block or the item goes up by one, so no two pieces meet in one slot.
-struct Parts {
-  int most;                               // parts of a row, at most
-  int halves;                             // parts of a row in a slot: the tensor-core kernel's two groups of warps may share rows
-  int first_item, rows_item;
-  int kt, blocks;
-  long long first_tile, tiles;
-};
-__device__ __forceinline__ Parts parts_of(const Args& a, const Plan& p, int g, int hk) {
-  Parts x;
-  x.tiles = p.tiles[a.G];
-  x.blocks = blocks_used(a, x.tiles);
-  x.rows_item = rows_of_item(a, p.rows[g]);
-  x.halves = a.tc && x.rows_item == 128 ? 2 : 1;
-  x.kt = (p.keys[g] + a.key_tile - 1) / a.key_tile;
-  const int rt = (p.rows[g] + x.rows_item - 1) / x.rows_item;
-  x.first_item = p.items[g] + hk * rt;
-  x.first_tile = p.tiles[g] + (long long)hk * rt * x.kt;
-  // an item of kt tiles meets at most this many shares of tiles / blocks
-  x.most = x.kt == 0 ? 0 : x.halves * (int)min((long long)x.blocks, ((long long)x.kt * x.blocks + x.tiles - 1) / x.tiles + 1);
-  return x;
-}
-// The workspace's row of part j of row n, or -1: it has no such part.
-__device__ __forceinline__ long long part_row(const Args& a, const Parts& x, int n, int j) {
-  const int i = n / x.rows_item;
-  const long long begin = x.first_tile + (long long)i * x.kt;
-  const int half = x.halves == 2 ? j & 1 : 0, b = block_of(begin, x.blocks, x.tiles) + (x.halves == 2 ? j >> 1 : j);
-  if (b > block_of(begin + x.kt - 1, x.blocks, x.tiles) || b + x.first_item + i >= a.slots) return -1;
-  return (long long)(b + x.first_item + i) * a.slot_rows + half * 128 + n % x.rows_item;
-}
-// (room for the weights of a row's parts)
-static inline int most_parts(const Args& a) { return (a.tc ? 2 : 1) * a.n_blocks; }
-
-__device__ __forceinline__ int group_of(const Args& a, const Plan& p, int t) {
-  if (t < a.group_start[0] || t >= a.group_start[a.G]) return -1;
-  int lo = 0, hi = a.G;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.t0[mid] <= t) lo = mid; else hi = mid;
-  }
-  if (t - p.t0[lo] < p.rows[lo] / (a.H / a.Hkv)) return lo;
-  flag_index(a);                          // (starts that do not ascend)
-  return -1;
-}
-// Whether a piece has a slot.  It has, unless the groups' starts do not ascend and their tokens overlap.
+// The piece that block b finds of item i lies in slot b + i of the workspace: along the shares either the block or the item
+// goes up by one, so no two pieces meet in one slot.  Every piece has a slot, unless the groups' starts do not ascend and
+// their tokens overlap.
 __device__ __forceinline__ bool slot_ok(const Args& a, const Segment& s) {
   if (blockIdx.x + (long long)s.item < a.slots) return true;
   flag_index(a);
   return false;
+}
+// For the second launch: where a group's items begin (block 0 says it), and an item's first and last block (each says it
+// of itself).
+__device__ __forceinline__ void record_groups(const Args& a, const Plan& p) {
+  if (blockIdx.x == 0)
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) a.first_item[g] = p.items[g];
+}
+__device__ __forceinline__ void record_item(const Args& a, const Segment& s) {
+  if (s.item >= a.slots) return;
+  if (s.tile == 0) a.item_blocks[s.item].x = blockIdx.x;
+  if ((s.tile + s.tiles) * a.key_tile >= s.keys) a.item_blocks[s.item].y = blockIdx.x;
+}
+// The parts of row n of a group and key head.
+struct Parts {
+  int n;                                  // how many
+  int halves;                             // of a slot's: two groups of warps of the tensor-core kernel share rows of few
+  long long slot;                         // the first one's slot
+  int row;                                // the row in a slot
+};
+__device__ __forceinline__ Parts parts_of(const Args& a, int g, int t0, int t1, int hk, int n) {
+  const int rows = (t1 - t0) * (a.H / a.Hkv), per = rows_of_item(a, rows);
+  const int item = a.first_item[g] + hk * ((rows + per - 1) / per) + n / per;
+  Parts x = {0, a.tc && per == 128 ? 2 : 1, 0, n % per};
+  if (item < 0 || item >= a.slots) return x;
+  const int2 b = a.item_blocks[item];
+  if (b.x < 0 || b.y < b.x || b.y >= a.n_blocks) return x;       // (a first launch that gave up)
+  x.n = x.halves * (b.y - b.x + 1);
+  x.slot = (long long)b.x + item;
+  return x;
+}
+// The workspace's row of part j, or -1: there is no such slot.
+__device__ __forceinline__ long long part_row(const Args& a, const Parts& x, int j) {
+  const long long slot = x.slot + (x.halves == 2 ? j >> 1 : j);
+  return slot < 0 || slot >= a.slots ? -1 : slot * a.slot_rows + (x.halves == 2 ? (j & 1) * 128 : 0) + x.row;
 }
 
 // eight entries of a row; vec: it begins on 16 bytes
@@ -232,6 +233,29 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, int vec, float (&v
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = __bfloat162float(p[i]);
+  }
+}
+__device__ __forceinline__ void store8(float* p, int vec, const float (&v)[8]) {
+  if (vec) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, int vec, const float (&v)[8]) {
+  if (vec) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) p[i] = __float2bfloat16_rn(v[i]);
   }
 }
 }  // namespace prefix

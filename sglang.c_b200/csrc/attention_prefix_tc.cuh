@@ -111,6 +111,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
   pdl_wait();
   pdl_launch_dependents();                          // (not before: the second launch reads what came before this one)
   make_plan(a, plan);
+  record_groups(a, plan);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -345,6 +346,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
         ok = mbar_wait(&ctl.o_full[w], o_turn++ & 1, abort_flag);
         tc_fence_after_sync();
       }
+      if (threadIdx.x == 0) record_item(a, s);
       if (busy && ok) {
         const long long at = (long long)(blockIdx.x + s.item) * TC_SLOT + (pair ? 0 : w * TC_WG) + mine;
         const bool there = valid && slot_ok(a, s);
