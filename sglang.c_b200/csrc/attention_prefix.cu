@@ -41,9 +41,9 @@ prefix_general_kernel(const Args a) {
   make_plan(a, plan);
   record_groups(a, plan);
   const float c2 = a.scale * LOG2E;
-  const int gq = a.H / a.Hkv;
+  const int gq = a.gq;
   for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
-    const int row0 = s.row_tile * GR, rows = min(GR, s.n_rows - row0);
+    const int row0 = s.row0, rows = min(GR, s.n_rows - row0), req = keeper(a, s);
     __syncthreads();
     for (int x = tid; x < GR * (D / 8); x += GT) {
       const int row = x / (D / 8), d = x % (D / 8) * 8;
@@ -77,7 +77,7 @@ prefix_general_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 8; i++) k[i] = v[i] = 0.0f;
         if (d < D && key < s.keys) {
-          const int page = page_of(a, s.req, key);
+          const int page = page_of(a, req, key);
           if (page >= 0) {
             const size_t at = row_at(a, page, s.hk, key) + d;
             load8(reinterpret_cast<const T*>(a.cache) + at, 1, k);
@@ -194,19 +194,18 @@ prefix_general_kernel(const Args a) {
 // keys of a round are asked for together.
 constexpr int OT = 128;
 
+constexpr int OWN_ONE = 16, OWN_TWO = 4;    // items a multiprocessor from which an item has one warp, two
+
 // Eight entries as they lie in memory.
 template <typename T> struct Raw;
 template <> struct Raw<__nv_bfloat16> {
   uint4 x;
   __device__ __forceinline__ void take(const __nv_bfloat16* p) { x = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void zero() { x = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; i++) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
 };
 template <> struct Raw<float> {
@@ -216,48 +215,55 @@ template <> struct Raw<float> {
     y = *reinterpret_cast<const float4*>(p + 4);
   }
   __device__ __forceinline__ void zero() { x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    v[0] = make_float2(x.x, x.y);
+    v[1] = make_float2(x.z, x.w);
+    v[2] = make_float2(y.x, y.y);
+    v[3] = make_float2(y.z, y.w);
   }
 };
 
 // A part of a softmax: maximum (times log2 e), sum of weights, and eight columns of the weighted sum.
 struct State {
-  float m, l, o[8];
-  __device__ __forceinline__ void join(float m2, float l2, const float (&o2)[8]) {
-    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top, f = exp2f(m - ref), f2 = exp2f(m2 - ref);
+  float m, l;
+  float2 o[4];
+  __device__ __forceinline__ void join(float m2, float l2, const float2 (&o2)[4]) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top, f = ex2(m - ref), f2 = ex2(m2 - ref);
     m = top;
     l = l * f + l2 * f2;
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = o[i] * f + o2[i] * f2;
+    for (int i = 0; i < 4; i++) o[i] = make_float2(o[i].x * f + o2[i].x * f2, o[i].y * f + o2[i].y * f2);
   }
 };
 
-// LW: lanes of a row, or 0: a.lanes.  warps: 1 or 4 of an item.
-template <typename T, int HC, int LW>
+// Keys of a walker a round: as many scores (keys x heads) as the walker has lanes, within what the registers hold.
+__host__ __device__ constexpr int round_keys(int size, int HC, int LW) {
+  const int most = 4 / (size == 4 ? 2 : 1), fit = LW / HC;
+  return fit < most ? fit : most;
+}
+
+// LW: lanes of a row.  WARPS: of an item; a block has four.
+template <typename T, int HC, int LW, int WARPS>
 __global__ void __launch_bounds__(OT)
-prefix_own_kernel(const Args a, int warps) {
-  extern __shared__ __align__(16) float sm[];          // [4 warps][HC][D + 2], for items of four warps
-  const int D = a.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = a.H / a.Hkv;
-  const int width = LW ? LW : a.lanes, of_warp = lane / width, sub = lane % width, per_warp = 32 / width;
+prefix_own_kernel(const Args a) {
+  extern __shared__ __align__(16) float sm[];          // [4 warps][HC][D + 2], then [HC][warps of an item]: for items of several
+  constexpr int per_warp = 32 / LW, ITEMS = 4 / WARPS;
+  const int D = a.D, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = a.gq;
+  const int of_warp = lane / LW, sub = lane % LW;
   const int share = blockIdx.z, shares = gridDim.z;
   if (shares > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_launch_dependents();
-  const int chunks = a.H / HC;
-  const long long item = warps == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
-  const bool real = item < (long long)a.T * chunks;
-  const int t = real ? (int)(item / chunks) : 0, h0 = (int)(item - (long long)t * chunks) * HC, hk = real ? h0 / gq : 0;
+  const int t = blockIdx.x * ITEMS + warp / WARPS, h0 = blockIdx.y * HC, hk = h0 / gq;
   // the token's group: the last one that begins at or before it
   int g = -1;
-  for (int x = 0; real && x < a.G; x += 32) g += __popc(__ballot_sync(0xffffffffu, x + lane < a.G && a.group_start[x + lane] <= t));
+  for (int x = 0; x < a.G; x += 32) g += __popc(__ballot_sync(0xffffffffu, x + lane < a.G && a.group_start[x + lane] <= t));
   int t0 = 0, t1 = 0;
   if (g >= 0) group_tokens(a, g, t0, t1);
   const bool inside = g >= 0 && t >= t0 && t < t1;
   // (starts that do not ascend, with the token behind this group's end and before the last one's)
-  if (g >= 0 && !inside && t < a.group_start[a.G]) flag_index(a);
-  const int keys = inside ? prefix_keys(a, g, t0, t1) : 0, walker = warps == 1 ? of_warp : (share * 4 + warp) * per_warp + of_warp;
-  const int walkers = (warps == 1 ? 1 : 4 * shares) * per_warp, d = sub * 8;
+  if (g >= 0 && !inside && t < min(a.group_start[a.G], a.T)) flag_index(a);
+  const int keys = inside ? prefix_length(a, g) : 0, walker = (share * WARPS + warp % WARPS) * per_warp + of_warp;
+  const int walkers = WARPS * shares * per_warp, d = sub * 8;
   const bool cols = d < D;
   State st[HC];
 #pragma unroll
@@ -265,86 +271,115 @@ prefix_own_kernel(const Args a, int warps) {
     st[h].m = -INFINITY;
     st[h].l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) st[h].o[i] = 0.0f;
+    for (int i = 0; i < 4; i++) st[h].o[i] = make_float2(0.0f, 0.0f);
   }
   if (inside) {
     const float c2 = a.scale * LOG2E;
     const int pos = a.positions[t], req = request_of(a, t);
     if (pos > a.last_position) flag_index(a);
     const int end = req < 0 ? keys : min(pos, a.last_position) + 1;          // own keys: keys .. end - 1
-    float q[HC][8];
+    float2 q[HC][4];
 #pragma unroll
     for (int h = 0; h < HC; h++) {
+      float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) q[h][i] = 0.0f;
-      if (cols) load8(reinterpret_cast<const T*>(a.q) + (size_t)t * a.q_stride + (size_t)(h0 + h) * D + d, a.q_vec, q[h]);
+      for (int i = 0; i < 8; i++) x[i] = 0.0f;
+      if (cols) load8(reinterpret_cast<const T*>(a.q) + (size_t)t * a.q_stride + (size_t)(h0 + h) * D + d, a.q_vec, x);
+#pragma unroll
+      for (int i = 0; i < 4; i++) q[h][i] = make_float2(x[2 * i], x[2 * i + 1]);
     }
-    constexpr int U = sizeof(T) == 2 && HC < 4 ? 4 : 2;          // keys of a walker a round
+    // A round: U keys' scores with HC heads are NV sums over the walker's lanes.  They are summed by halves: at each of the
+    // first levels a lane keeps one half of the sums and gives its part of the others away, so that NV sums take
+    // NV - 1 shuffles and a lane has one at the end, number sub / COPIES; it makes that one's weight, and the weights go round.
+    constexpr int U = round_keys(sizeof(T), HC, LW), NV = U * HC, COPIES = LW / NV;
+    const int my_u = sub / COPIES / HC, base = lane & ~(LW - 1);
+    float m = -INFINITY, l = 0.0f;                     // of this lane's head; weights of its place among the sums only
     const size_t v_at = value_offset(a);
     // 32 pages at a time, a lane an id
-    for (int block0 = (unsigned)keys / (unsigned)a.page_size; (long long)block0 * a.page_size < end; block0 += 32) {
+    for (int block0 = block_in(a, keys); (long long)block0 * a.page_size < end; block0 += 32) {
       const long long stop = min((long long)end, (long long)(block0 + 32) * a.page_size);
       const int first = max(keys, block0 * a.page_size), last = (int)stop;
       const int id = (long long)(block0 + lane) * a.page_size < last ? page_of(a, req, (block0 + lane) * a.page_size) : -1;
       for (int key0 = first + (walker - of_warp) * U; key0 < last; key0 += walkers * U) {
         // (the bounds are the warp's: its lanes take the shuffles together)
         Raw<T> k[U], v[U];
-        bool in[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          const int key = key0 + u * per_warp + of_warp;
-          const int page = __shfl_sync(0xffffffffu, id, ((unsigned)key / (unsigned)a.page_size - block0) & 31);
-          in[u] = key < last;
+          const int key = key0 + u * per_warp + of_warp, block = block_in(a, key);
+          const int page = __shfl_sync(0xffffffffu, id, (block - block0) & 31);
           k[u].zero();
           v[u].zero();
-          if (in[u] && page >= 0 && cols) {
-            const T* x = reinterpret_cast<const T*>(a.cache) + row_at(a, page, hk, key) + d;
+          if (key < last && page >= 0 && cols) {
+            const T* x = reinterpret_cast<const T*>(a.cache) + (((size_t)page * 2 * a.Hkv + hk) * a.page_size + (key - block * a.page_size)) * D + d;
             k[u].take(x);
             v[u].take(x + v_at);
           }
         }
+        float s[NV];
 #pragma unroll
-        for (int h = 0; h < HC; h++) {
-          float s[U], mx = -INFINITY;
+        for (int u = 0; u < U; u++) {
+          float2 x[4];
+          k[u].get(x);
 #pragma unroll
-          for (int u = 0; u < U; u++) {
-            float x[8];
-            k[u].get(x);
-            s[u] = 0.0f;
+          for (int h = 0; h < HC; h++) {
+            float2 e = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < 8; i++) s[u] = fmaf(q[h][i], x[i], s[u]);
+            for (int i = 0; i < 4; i++) e = fma2(q[h][i], x[i], e);
+            s[u * HC + h] = e.x + e.y;
           }
+        }
 #pragma unroll
-          for (int w = 1; w < (LW ? LW : 32); w <<= 1) {
-            if (!LW && w >= width) break;
+        for (int w = LW / 2, n = NV; w > 0; w >>= 1) {
+          const bool up = sub & w;
+          if (n > 1) {
+            n >>= 1;
 #pragma unroll
-            for (int u = 0; u < U; u++) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+            for (int i = 0; i < NV / 2; i++)
+              if (i < n) {
+                const float give = up ? s[i] : s[n + i], keep = up ? s[n + i] : s[i];
+                s[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+              }
+          } else {
+            s[0] += __shfl_xor_sync(0xffffffffu, s[0], w);
           }
+        }
+        float score = key0 + my_u * per_warp + of_warp < last ? s[0] * c2 : -INFINITY, top = score;
 #pragma unroll
-          for (int u = 0; u < U; u++) {
-            s[u] = in[u] ? s[u] : -INFINITY;
-            mx = fmaxf(mx, s[u]);
+        for (int w = LW / 2; w >= HC * COPIES; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        top = fmaxf(top, m);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        if (__any_sync(0xffffffffu, top > m)) {
+          const float f = ex2(m - ref);                // (0 where nothing was seen before)
+          l *= f;
+          m = top;
+#pragma unroll
+          for (int h = 0; h < HC; h++) {
+            const float fh = __shfl_sync(0xffffffffu, f, base + h * COPIES);
+#pragma unroll
+            for (int i = 0; i < 4; i++) st[h].o[i] = make_float2(st[h].o[i].x * fh, st[h].o[i].y * fh);
           }
-          mx *= c2;
-          if (mx > st[h].m) {
-            const float f = exp2f(st[h].m - mx);
-            st[h].m = mx;
-            st[h].l *= f;
+        }
+        const float p = ex2(score - ref);
+        l += p;
 #pragma unroll
-            for (int i = 0; i < 8; i++) st[h].o[i] *= f;
-          }
-          const float ref = st[h].m == -INFINITY ? 0.0f : st[h].m;
+        for (int u = 0; u < U; u++) {
+          float2 x[4];
+          v[u].get(x);
 #pragma unroll
-          for (int u = 0; u < U; u++) {
-            const float p = exp2f(fmaf(s[u], c2, -ref));
-            float x[8];
-            v[u].get(x);
-            st[h].l += p;
+          for (int h = 0; h < HC; h++) {
+            const float ph = __shfl_sync(0xffffffffu, p, base + (u * HC + h) * COPIES);
 #pragma unroll
-            for (int i = 0; i < 8; i++) st[h].o[i] = fmaf(p, x[i], st[h].o[i]);
+            for (int i = 0; i < 4; i++) st[h].o[i] = fma2(make_float2(ph, ph), x[i], st[h].o[i]);
           }
         }
       }
+    }
+#pragma unroll
+    for (int w = LW / 2; w >= HC * COPIES; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+#pragma unroll
+    for (int h = 0; h < HC; h++) {
+      st[h].m = __shfl_sync(0xffffffffu, m, base + h * COPIES);
+      st[h].l = __shfl_sync(0xffffffffu, l, base + h * COPIES);
     }
   }
   pdl_wait();                                          // the prefixes' parts are there
@@ -353,90 +388,101 @@ prefix_own_kernel(const Args a, int warps) {
     for (int j = walker; j < ps.n; j += walkers) {
       const long long at = part_row(a, ps, j);
       if (at < 0) continue;
+      float2 ml[HC], o[HC][4];
 #pragma unroll
       for (int h = 0; h < HC; h++) {
-        const float2 ml = a.part_ml[at + h];
-        if (ml.y == 0.0f) continue;                    // nothing was seen and no sums were written (NaN is not 0)
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = 0.0f;
-        if (cols) load8(a.part_o + (at + h) * D + d, 1, o);
-        st[h].join(ml.x, ml.y, o);
+        Raw<float> x;
+        x.zero();
+        ml[h] = a.part_ml[at + h];
+        if (cols) x.take(a.part_o + (at + h) * D + d);
+        x.get(o[h]);
       }
+#pragma unroll
+      for (int h = 0; h < HC; h++)
+        if (ml[h].y != 0.0f) st[h].join(ml[h].x, ml[h].y, o[h]);       // (0: nothing was seen and no sums were written; NaN is not 0)
     }
   }
   // the warp's walkers
 #pragma unroll
   for (int h = 0; h < HC; h++)
 #pragma unroll
-    for (int w = 16; w >= (LW ? LW : 1); w >>= 1) {
-      if (!LW && w < width) break;
-      float o[8];
+    for (int w = 16; w >= LW; w >>= 1) {
+      float2 o[4];
       const float m = __shfl_xor_sync(0xffffffffu, st[h].m, w), l = __shfl_xor_sync(0xffffffffu, st[h].l, w);
 #pragma unroll
-      for (int i = 0; i < 8; i++) o[i] = __shfl_xor_sync(0xffffffffu, st[h].o[i], w);
+      for (int i = 0; i < 4; i++)
+        o[i] = make_float2(__shfl_xor_sync(0xffffffffu, st[h].o[i].x, w), __shfl_xor_sync(0xffffffffu, st[h].o[i].y, w));
       st[h].join(m, l, o);
     }
-  if (warps == 1) {
+  if constexpr (WARPS == 1) {
     if (inside && of_warp == 0 && cols) {
 #pragma unroll
       for (int h = 0; h < HC; h++) {
         const float f = st[h].l == 0.0f ? 0.0f : 1.0f / st[h].l;
         float o[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = st[h].l == 0.0f ? 0.0f : st[h].o[i] * f;
+        for (int i = 0; i < 8; i++) o[i] = st[h].l == 0.0f ? 0.0f : (i & 1 ? st[h].o[i / 2].y : st[h].o[i / 2].x) * f;
         store8(reinterpret_cast<T*>(a.out) + (size_t)t * a.o_stride + (size_t)(h0 + h) * D + d, a.o_vec, o);
       }
     }
-    return;
-  }
-  // the block's warps, and the cluster's blocks
-  const int one = HC * (D + 2);
-  if (of_warp == 0) {
+  } else {
+    // the item's warps, and the cluster's blocks
+    const int one = HC * (D + 2), parts = WARPS * shares, warp0 = warp / WARPS * WARPS, mine = threadIdx.x % (WARPS * 32);
+    if (of_warp == 0) {
 #pragma unroll
-    for (int h = 0; h < HC; h++) {
-      float* to = sm + warp * one + h * (D + 2);
-      if (cols)
+      for (int h = 0; h < HC; h++) {
+        float* to = sm + warp * one + h * (D + 2);
+        if (cols)
 #pragma unroll
-        for (int i = 0; i < 8; i++) to[d + i] = st[h].o[i];
-      if (sub == 0) {
-        to[D] = st[h].m;
-        to[D + 1] = st[h].l;
+          for (int i = 0; i < 8; i++) to[d + i] = i & 1 ? st[h].o[i / 2].y : st[h].o[i / 2].x;
+        if (sub == 0) {
+          to[D] = st[h].m;
+          to[D + 1] = st[h].l;
+        }
       }
     }
-  }
-  if (shares > 1) {
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // (of the start)
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  } else {
-    __syncthreads();
-  }
-  if (share == 0 && inside) {
-    auto other = [&](int z, int i) {                   // word i of warp z of the cluster
-      if (z < 4) return sm[z * one + i];
+    if (shares > 1) {
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // (of the start)
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+      __syncthreads();
+    }
+    auto other = [&](int z, int i) {                   // word i of warp z of the item
+      const float* at = sm + (warp0 + z % WARPS) * one + i;
+      if (z < WARPS) return *at;
       uint32_t there;
       float v;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(sm + (z & 3) * one + i)), "r"(z >> 2));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(z / WARPS));
       asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
       return v;
     };
-    for (int x = threadIdx.x; x < HC * D; x += OT) {
-      const int h = x / D, c = x - h * D, at = h * (D + 2);
-      float M = -INFINITY, sum = 0.0f, total = 0.0f;
-      for (int z = 0; z < 4 * shares; z++) M = fmaxf(M, other(z, at + D));
+    float* factor = sm + 4 * one + warp0 * HC * shares;
+    if (share == 0 && mine < HC) {
+      const int at = mine * (D + 2) + D;
+      float M = -INFINITY, total = 0.0f;
+      for (int z = 0; z < parts; z++) M = fmaxf(M, other(z, at));
       const float ref = M == -INFINITY ? 0.0f : M;
-      for (int z = 0; z < 4 * shares; z++) {
-        const float f = exp2f(other(z, at + D) - ref);
-        sum = fmaf(f, other(z, at + c), sum);
-        total = fmaf(f, other(z, at + D + 1), total);
+      for (int z = 0; z < parts; z++) {
+        const float f = ex2(other(z, at) - ref);
+        factor[mine * parts + z] = f;
+        total = fmaf(f, other(z, at + 1), total);
       }
-      reinterpret_cast<T*>(a.out)[(size_t)t * a.o_stride + (size_t)(h0 + h) * D + c] = from_f32<T>(total == 0.0f ? 0.0f : sum / total);
+      const float f = total == 0.0f ? 0.0f : 1.0f / total;
+      for (int z = 0; z < parts; z++) factor[mine * parts + z] *= f;
     }
-  }
-  if (shares > 1) {                                    // (block 0 has read the others' shared memory)
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncthreads();
+    if (share == 0 && inside)
+      for (int x = mine; x < HC * D; x += WARPS * 32) {
+        const int h = x / D, c = x - h * D;
+        float sum = 0.0f;
+        for (int z = 0; z < parts; z++) sum = fmaf(factor[h * parts + z], other(z, h * (D + 2) + c), sum);
+        reinterpret_cast<T*>(a.out)[(size_t)t * a.o_stride + (size_t)(h0 + h) * D + c] = from_f32<T>(sum);
+      }
+    if (shares > 1) {                                  // (block 0 has read the others' shared memory)
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
   }
 }
 
@@ -458,31 +504,42 @@ int run_general(const Args& a, cudaStream_t stream) {
   }
 }
 
-template <typename T, int HC, int LW>
-int launch_own(const Args& a, int warps, int shares, cudaStream_t stream) {
-  const size_t smem = warps == 1 ? 0 : (size_t)4 * HC * (a.D + 2) * 4;
-  const long long items = (long long)a.T * (a.H / HC);
-  return sglc_launch(prefix_own_kernel<T, HC, LW>, dim3((unsigned)(warps == 1 ? (items + 3) / 4 : items), 1, shares), dim3(OT), smem,
-                     stream, shares, true, a, warps);
+template <typename T, int HC, int LW, int WARPS>
+int launch_own(const Args& a, int shares, cudaStream_t stream) {
+  const size_t smem = WARPS == 1 ? 0 : (size_t)(4 * HC * (a.D + 2) + 4 * HC * shares) * 4;
+  return sglc_launch(prefix_own_kernel<T, HC, LW, WARPS>, dim3((a.T * WARPS + 3) / 4, a.H / HC, shares), dim3(OT), smem, stream, shares,
+                     true, a);
 }
-template <typename T, int HC>
-int choose_own(const Args& a, int warps, int shares, cudaStream_t stream) {
-  if (a.lanes == 8) return launch_own<T, HC, 8>(a, warps, shares, stream);
-  if (a.lanes == 16) return launch_own<T, HC, 16>(a, warps, shares, stream);
-  return launch_own<T, HC, 0>(a, warps, shares, stream);
+template <typename T, int HC, int LW>
+int warps_own(const Args& a, int max_own, cudaStream_t stream) {
+  // A warp an item where the items fill the multiprocessors' warps, else two, else four, and blocks of a cluster while
+  // there are fewer than four a multiprocessor and 64 keys or more are left for each.
+  const long long items = (long long)a.T * (a.H / HC);
+  if (items >= OWN_ONE * a.sms) return launch_own<T, HC, LW, 1>(a, 1, stream);
+  if (items >= OWN_TWO * a.sms) return launch_own<T, HC, LW, 2>(a, 1, stream);
+  int shares = 1;
+  while (shares < 8 && items * shares * 2 <= 4LL * a.sms && max_own >= 64 * shares * 2) shares *= 2;
+  return launch_own<T, HC, LW, 4>(a, shares, stream);
+}
+template <typename T, int LW>
+int choose_own(const Args& a, int max_own, cudaStream_t stream) {
+  const int gq = a.H / a.Hkv;
+  if constexpr (LW >= 4)
+    if (gq % 4 == 0) return warps_own<T, 4, LW>(a, max_own, stream);
+  if constexpr (LW >= 2)
+    if (gq % 2 == 0) return warps_own<T, 2, LW>(a, max_own, stream);
+  return warps_own<T, 1, LW>(a, max_own, stream);
 }
 template <typename T>
 int run_own(const Args& a, int max_own, cudaStream_t stream) {
-  const int gq = a.H / a.Hkv, hc = gq % 4 == 0 ? 4 : gq % 2 == 0 ? 2 : 1;
-  const long long items = (long long)a.T * (a.H / hc);
-  // A warp an item where the items fill the multiprocessors and their own keys are few; else four, and blocks of a
-  // cluster while there are fewer than four a multiprocessor and 64 keys or more are left for each.
-  const int warps = items >= 16LL * a.sms && max_own <= 128 ? 1 : 4;
-  int shares = 1;
-  while (warps == 4 && shares < 8 && items * shares * 2 <= 4LL * a.sms && max_own >= 64 * shares * 2) shares *= 2;
-  if (hc == 4) return choose_own<T, 4>(a, warps, shares, stream);
-  if (hc == 2) return choose_own<T, 2>(a, warps, shares, stream);
-  return choose_own<T, 1>(a, warps, shares, stream);
+  switch (a.lanes) {
+    case 1: return choose_own<T, 1>(a, max_own, stream);
+    case 2: return choose_own<T, 2>(a, max_own, stream);
+    case 4: return choose_own<T, 4>(a, max_own, stream);
+    case 8: return choose_own<T, 8>(a, max_own, stream);
+    case 16: return choose_own<T, 16>(a, max_own, stream);
+    default: return choose_own<T, 32>(a, max_own, stream);
+  }
 }
 
 int multiprocessors() {
@@ -498,8 +555,10 @@ bool lay_out(Args* a, int dtype) {
   a->tc = dtype == SGLC_BF16 && (a->D == 64 || a->D == 128);
   a->n_blocks = a->tc ? a->sms : 2 * a->sms;
   a->slot_rows = a->tc ? TC_SLOT : GENERAL_ROWS;
-  a->key_tile = a->tc ? TC_KEYS : GENERAL_KEYS;
-  const long long rows = (long long)a->T * (a->H / a->Hkv);
+  a->gq = a->H / a->Hkv;
+  a->key_shift = a->tc ? 7 : 6;
+  static_assert(TC_KEYS == 128 && GENERAL_KEYS == 64 && GENERAL_ROWS == 64, "as the shifts say");
+  const long long rows = (long long)a->T * a->gq;
   a->slots = a->n_blocks + a->Hkv * (rows / a->slot_rows + a->G);      // (items of 128 rows are the only ones of their group)
   a->lanes = 1;
   while (a->lanes * 8 < a->D) a->lanes *= 2;
@@ -508,7 +567,7 @@ bool lay_out(Args* a, int dtype) {
 // floats of workspace: the parts' sums, their (maximum, sum of weights), the groups' first items, the items' blocks
 long long words(const Args& a) { return a.slots * a.slot_rows * (a.D + 2) + (a.G + 1) / 2 * 2 + 2 * a.slots; }
 bool sizes_ok(int T, int R, int G, int H, int Hkv, int D) {
-  return T >= 0 && R >= 0 && G >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && D > 0;
+  return T >= 0 && R >= 0 && G >= 0 && H > 0 && H <= 65535 && Hkv > 0 && H % Hkv == 0 && D > 0;
 }
 }  // namespace
 
@@ -544,6 +603,7 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   a.out = out; a.o_stride = o_stride;
   a.T = T; a.G = G; a.H = H; a.Hkv = Hkv; a.D = D; a.page_size = page_size; a.n_pages = n_pages; a.scale = scale;
   const long long room = (long long)bt_width * page_size;
+  a.page_shift = page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size);
   a.last_position = (int)(room > 0x7ffffff0LL ? 0x7ffffff0LL : room) - 1;
   a.err = err;
   if (!lay_out(&a, dtype)) return SGLC_ERR_ARGUMENT;

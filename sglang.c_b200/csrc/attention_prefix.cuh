@@ -19,17 +19,18 @@ struct Args {
   void* out;
   long long o_stride;
   int o_vec;                              // (so can rows of results)
-  int T, R, G, H, Hkv, D, page_size, n_pages;
+  int T, R, G, H, Hkv, gq, D, page_size, n_pages;        // gq: query heads of a key head
+  int page_shift;                         // log2 of the page size, or -1
   int last_position;                      // the last one that a row of the table has room for
   float scale;
   int* err;
   // the launch
-  int sms, n_blocks, slot_rows, key_tile, lanes;
+  int sms, n_blocks, slot_rows, key_shift, lanes;        // key_shift: log2 of a tile's keys
   int tc;                                 // the tensor-core kernel
   long long slots;
   float* part_o;                          // [slots][slot_rows][D]: sums, against a maximum
   float2* part_ml;                        // [slots][slot_rows]: that maximum (times log2 e), sum of weights
-  int* first_item;                        // [G]: items of the groups before
+  int* first_item;                        // [G]: items of the groups before, or -1: no prefix, or one that no request names
   int2* item_blocks;                      // [slots]: the first and the last block that has a piece of the item
 };
 
@@ -49,14 +50,18 @@ __device__ __forceinline__ int request_of(const Args& a, int t) {
   flag_index(a);
   return -1;
 }
+__device__ __forceinline__ int block_in(const Args& a, int key) {
+  return a.page_shift >= 0 ? key >> a.page_shift : (int)((unsigned)key / (unsigned)a.page_size);
+}
 __device__ __forceinline__ int page_of(const Args& a, int req, int key) {
-  const int page = a.table[(size_t)req * a.bt_stride + (unsigned)key / (unsigned)a.page_size];
+  if (req < 0) return -1;
+  const int page = a.table[(size_t)req * a.bt_stride + block_in(a, key)];
   if (page >= 0 && page < a.n_pages) return page;
   flag_index(a);
   return -1;
 }
 __device__ __forceinline__ size_t row_at(const Args& a, int page, int hk, int key) {
-  return (((size_t)page * 2 * a.Hkv + hk) * a.page_size + (unsigned)key % (unsigned)a.page_size) * a.D;
+  return (((size_t)page * 2 * a.Hkv + hk) * a.page_size + (key - block_in(a, key) * a.page_size)) * a.D;
 }
 __device__ __forceinline__ size_t value_offset(const Args& a) { return (size_t)a.Hkv * a.page_size * a.D; }
 // keys of a prefix of `keys` that token t sees
@@ -67,28 +72,28 @@ __device__ __forceinline__ void group_tokens(const Args& a, int g, int& t0, int&
   t0 = min(max(a.group_start[g], 0), a.T);
   t1 = min(max(a.group_start[g + 1], t0), a.T);
 }
-__device__ __forceinline__ int prefix_keys(const Args& a, int g, int t0, int t1) {
-  const int keys = t1 > t0 ? min(max(a.shared_len[g], 0), a.last_position + 1) : 0;
-  return keys > 0 && request_of(a, t0) < 0 ? 0 : keys;
-}
+__device__ __forceinline__ int prefix_length(const Args& a, int g) { return min(max(a.shared_len[g], 0), a.last_position + 1); }
 
-// Rows of an item of a group of so many rows a key head.
-__device__ __forceinline__ int rows_of_item(const Args& a, int rows) { return a.tc && rows <= 128 ? 128 : a.slot_rows; }
+// Rows of an item of a group of so many rows a key head, as a power of two.
+__device__ __forceinline__ int item_shift(const Args& a, int rows) { return !a.tc ? 6 : rows <= 128 ? 7 : 8; }
+__device__ __forceinline__ int items_of(const Args& a, int rows) { return (int)(((long long)rows + (1 << item_shift(a, rows)) - 1) >> item_shift(a, rows)); }
+__device__ __forceinline__ int tiles_of_keys(const Args& a, int keys) { return (keys + (1 << a.key_shift) - 1) >> a.key_shift; }
+// (a division of 64 bits takes a hundred instructions)
+__device__ __forceinline__ long long divide(long long x, int y) {
+  return (unsigned long long)x >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
+}
 
 // Every thread of the block calls it.
 __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
-  const int gq = a.H / a.Hkv;
   for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
+    const int length = prefix_length(a, g);
     int t0, t1;
     group_tokens(a, g, t0, t1);
-    const int keys = prefix_keys(a, g, t0, t1);
+    const int keys = t1 > t0 ? length : 0;
     p.t0[g] = t0;
     p.keys[g] = keys;
-    p.rows[g] = (t1 - t0) * gq;
-    const int per = rows_of_item(a, p.rows[g]);
-    const int items = keys > 0 ? a.Hkv * ((p.rows[g] + per - 1) / per) : 0;
-    p.items[g + 1] = items;
-    p.tiles[g + 1] = (long long)items * ((keys + a.key_tile - 1) / a.key_tile);
+    p.rows[g] = (t1 - t0) * a.gq;
+    p.items[g + 1] = keys > 0 ? a.Hkv * items_of(a, p.rows[g]) : 0;
   }
   __syncthreads();
   if (threadIdx.x < 32) {                 // sums over the groups before
@@ -97,9 +102,8 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
     for (int g0 = 0; g0 < a.G; g0 += 32) {
       const int g = g0 + threadIdx.x;
       int x = g < a.G ? p.items[g + 1] : 0;
-      long long y = g < a.G ? p.tiles[g + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
+      long long y = g < a.G ? (long long)x * tiles_of_keys(a, p.keys[g]) : 0;
+      for (int o = 1; o < 32 && o < a.G; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, x, o);
         const long long v = __shfl_up_sync(0xffffffffu, y, o);
         if ((int)threadIdx.x >= o) {
@@ -111,8 +115,9 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
         p.items[g + 1] = items + x;
         p.tiles[g + 1] = tiles + y;
       }
-      items += __shfl_sync(0xffffffffu, x, 31);
-      tiles += __shfl_sync(0xffffffffu, y, 31);
+      const int last = min(31, a.G - 1 - g0);
+      items += __shfl_sync(0xffffffffu, x, last);
+      tiles += __shfl_sync(0xffffffffu, y, last);
     }
     if (threadIdx.x == 0) p.items[0] = 0, p.tiles[0] = 0;
   }
@@ -125,9 +130,9 @@ __device__ __forceinline__ int blocks_used(const Args& a, long long tiles) { ret
 
 // A block's piece of an item.
 struct Segment {
-  int g, item, hk, row_tile;              // group; item counted over all groups; its key head and rows
-  int rows_item;                          // rows of an item of its group
-  int t0, n_rows, keys, req;              // the group's first token, rows a key head, prefix, and whose pages hold it
+  int item, hk, row0;                     // item counted over all groups; its key head and first row of that
+  int t0, n_rows, keys;                   // the group's first token, rows a key head, prefix
+  int shift;                              // log2 of an item's rows
   int tile, tiles;                        // tiles of keys: the first, how many
   long long at, end;                      // the piece's first tile and the end of the block's share, counted over all items
 };
@@ -142,30 +147,31 @@ __device__ __forceinline__ Segment segment_at(const Args& a, const Plan& p, long
     const int mid = (lo + hi) >> 1;
     if (p.tiles[mid] <= at) lo = mid; else hi = mid;
   }
-  s.g = lo;
   s.t0 = p.t0[lo];
   s.n_rows = p.rows[lo];
   s.keys = p.keys[lo];
-  s.req = a.token_req ? a.token_req[s.t0] : s.t0;
-  s.rows_item = rows_of_item(a, s.n_rows);
-  const int kt = (s.keys + a.key_tile - 1) / a.key_tile, rt = (s.n_rows + s.rows_item - 1) / s.rows_item;
-  const int n = (int)((at - p.tiles[lo]) / kt);
-  s.tile = (int)((at - p.tiles[lo]) % kt);
+  s.shift = item_shift(a, s.n_rows);
+  const int kt = tiles_of_keys(a, s.keys), rt = items_of(a, s.n_rows);
+  const int n = (int)divide(at - p.tiles[lo], kt);
+  s.tile = (int)(at - p.tiles[lo] - (long long)n * kt);
   s.tiles = (int)min((long long)(kt - s.tile), end - at);
   s.item = p.items[lo] + n;
-  s.hk = n / rt;
-  s.row_tile = n % rt;
+  s.hk = (unsigned)n / (unsigned)rt;
+  s.row0 = (n - s.hk * rt) << s.shift;
   return s;
 }
 __device__ __forceinline__ Segment first_segment(const Args& a, const Plan& p) {
   const long long tiles = p.tiles[a.G];
   const int blocks = blocks_used(a, tiles);
   if ((int)blockIdx.x >= blocks) return segment_at(a, p, 0, 0);
-  return segment_at(a, p, tiles * blockIdx.x / blocks, tiles * (blockIdx.x + 1) / blocks);
+  return segment_at(a, p, divide(tiles * blockIdx.x, blocks), divide(tiles * (blockIdx.x + 1), blocks));
 }
 __device__ __forceinline__ Segment next_segment(const Args& a, const Plan& p, const Segment& s) {
   return segment_at(a, p, s.at + s.tiles, s.end);
 }
+
+// Whose pages hold a segment's keys: the request of the group's first token (-1: there is no such one).
+__device__ __forceinline__ int keeper(const Args& a, const Segment& s) { return s.tiles > 0 ? request_of(a, s.t0) : -1; }
 
 // The piece that block b finds of item i lies in slot b + i of the workspace: along the shares either the block or the item
 // goes up by one, so no two pieces meet in one slot.  Every piece has a slot, unless the groups' starts do not ascend and
@@ -179,12 +185,12 @@ __device__ __forceinline__ bool slot_ok(const Args& a, const Segment& s) {
 // of itself).
 __device__ __forceinline__ void record_groups(const Args& a, const Plan& p) {
   if (blockIdx.x == 0)
-    for (int g = threadIdx.x; g < a.G; g += blockDim.x) a.first_item[g] = p.items[g];
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) a.first_item[g] = p.keys[g] > 0 ? p.items[g] : -1;
 }
 __device__ __forceinline__ void record_item(const Args& a, const Segment& s) {
   if (s.item >= a.slots) return;
   if (s.tile == 0) a.item_blocks[s.item].x = blockIdx.x;
-  if ((s.tile + s.tiles) * a.key_tile >= s.keys) a.item_blocks[s.item].y = blockIdx.x;
+  if ((s.tile + s.tiles) << a.key_shift >= s.keys) a.item_blocks[s.item].y = blockIdx.x;
 }
 // The parts of row n of a group and key head.
 struct Parts {
@@ -194,10 +200,10 @@ struct Parts {
   int row;                                // the row in a slot
 };
 __device__ __forceinline__ Parts parts_of(const Args& a, int g, int t0, int t1, int hk, int n) {
-  const int rows = (t1 - t0) * (a.H / a.Hkv), per = rows_of_item(a, rows);
-  const int item = a.first_item[g] + hk * ((rows + per - 1) / per) + n / per;
-  Parts x = {0, a.tc && per == 128 ? 2 : 1, 0, n % per};
-  if (item < 0 || item >= a.slots) return x;
+  const int rows = (t1 - t0) * a.gq, shift = item_shift(a, rows);
+  const int first = a.first_item[g], item = first + hk * items_of(a, rows) + (n >> shift);
+  Parts x = {0, a.tc && shift == 7 ? 2 : 1, 0, n & ((1 << shift) - 1)};
+  if (first < 0 || item < 0 || item >= a.slots) return x;
   const int2 b = a.item_blocks[item];
   if (b.x < 0 || b.y < b.x || b.y >= a.n_blocks) return x;       // (a first launch that gave up)
   x.n = x.halves * (b.y - b.x + 1);
@@ -208,6 +214,20 @@ __device__ __forceinline__ Parts parts_of(const Args& a, int g, int t0, int t1, 
 __device__ __forceinline__ long long part_row(const Args& a, const Parts& x, int j) {
   const long long slot = x.slot + (x.halves == 2 ? j >> 1 : j);
   return slot < 0 || slot >= a.slots ? -1 : slot * a.slot_rows + (x.halves == 2 ? (j & 1) * 128 : 0) + x.row;
+}
+
+// 2^x by the special-function unit, 2 units in the last place (-inf gives 0)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two products and sums at a time, each rounded as one alone.
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y)),
+      "l"(reinterpret_cast<unsigned long long&>(z)));
+  return reinterpret_cast<float2&>(r);
 }
 
 // eight entries of a row; vec: it begins on 16 bytes

@@ -45,17 +45,6 @@ __device__ __forceinline__ void mma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, ui
       : "r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y)),
-      "l"(reinterpret_cast<unsigned long long&>(z)));
-  return reinterpret_cast<float2&>(r);
-}
 __device__ __forceinline__ float2 add2(float2 x, float2 y) {
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y)));
@@ -117,7 +106,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
   tc_fence_after_sync();
   const uint32_t tmem = ctl.tmem_base;
   volatile int* abort_flag = &ctl.abort_flag;
-  const int gq = a.H / a.Hkv;
+  const int gq = a.gq;
 
   if (warp >= TC_LOAD_WARP) {
     // ---- loads, a warp for keys and one for values: a lane a box, whose page is asked for a tile ahead ----
@@ -126,10 +115,11 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
     uint8_t* mine = ring + half * RING * UNIT;
     Segment s = first_segment(a, plan);
     int j = 0;
+    int req = keeper(a, s);
     auto page_id = [&](const Segment& x, int jj, int b) {
       const int key = (x.tile + jj) * TC_KEYS + b * box;
       if (x.tiles <= 0 || b * box >= TC_KEYS || key >= x.keys) return -1;
-      const int page = page_of(a, x.req, key);
+      const int page = page_of(a, req, key);
       return page < 0 ? a.n_pages : page;           // (a page outside reads as zeros)
     };
     int id_next = page_id(s, 0, lane);
@@ -154,6 +144,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       }
       if (++j == s.tiles) {
         s = next_segment(a, plan, s);
+        req = keeper(a, s);
         j = 0;
       }
       id_next = page_id(s, j, lane);
@@ -176,7 +167,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       uint32_t u0 = 0, q_turn = 0, turn = 0;
       bool ok = true;
       for (Segment s = first_segment(a, plan); s.tiles > 0 && ok; s = next_segment(a, plan, s)) {
-        const bool pair = s.rows_item == 2 * TC_WG;
+        const bool pair = s.shift == 8;
         const uint32_t q_at = smem_u32(sQ) + (pair ? w * UNIT : 0);
         ok = mbar_wait(&ctl.q_full, q_turn & 1, abort_flag);
         if (!ok) break;
@@ -232,31 +223,42 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
     uint32_t turn = 0, u0 = 0, o_turn = 0;          // steps, tiles and pieces so far
     bool ok = true;
     for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
-      const bool pair = s.rows_item == 2 * TC_WG;
-      const int rows = min(s.rows_item, s.n_rows - s.row_tile * s.rows_item);  // of this item
+      const bool pair = s.shift == 8;
+      const int rows = min(1 << s.shift, s.n_rows - s.row0);         // of this item
       const int mine = pair ? w * TC_WG + row : row;
-      const int n = s.row_tile * s.rows_item + mine, t = s.t0 + n / gq;
+      const int n = s.row0 + mine, t = s.t0 + (unsigned)n / (unsigned)gq;
       const bool valid = mine < rows;
       const int lim = valid ? visible(a, t, s.keys) : 0;
       // both groups are done with the item before (its products have been waited for): queries of this one
       asm volatile("bar.sync 1, 256;" ::: "memory");
       {
-        // (the same 128 rows for both groups: half of the columns each)
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)(s.hk * gq + n % gq) * D;
-        const int c0 = pair ? 0 : w * (D / 16), c1 = pair ? D / 8 : c0 + D / 16;
+        // (the same 128 rows for both groups: half of the columns each; all pieces asked for at once)
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)(s.hk * gq + n - (t - s.t0) * gq) * D;
+        const int c0 = pair ? 0 : w * (D / 16);
         uint8_t* dst = sQ + (pair ? w * UNIT : 0);
-        for (int c = c0; c < c1; c++) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (valid) {
-            if (a.q_vec) {
-              x = *reinterpret_cast<const uint4*>(src + c * 8);
-            } else {
-              const unsigned short* h = reinterpret_cast<const unsigned short*>(src + c * 8);
-              x = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                             h[6] | (uint32_t)h[7] << 16);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          uint4 x[D / 16];
+#pragma unroll
+          for (int c = 0; c < D / 16; c++) {
+            x[c] = make_uint4(0u, 0u, 0u, 0u);
+            const __nv_bfloat16* from = src + (c0 + half * (D / 16) + c) * 8;
+            if (valid && (pair || half == 0)) {
+              if (a.q_vec) {
+                x[c] = *reinterpret_cast<const uint4*>(from);
+              } else {
+                const unsigned short* h = reinterpret_cast<const unsigned short*>(from);
+                x[c] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                                  h[6] | (uint32_t)h[7] << 16);
+              }
             }
           }
-          *reinterpret_cast<uint4*>(dst + (c / 8) * TC_TILE + sw128(row, c % 8)) = x;
+          if (pair || half == 0)
+#pragma unroll
+            for (int c = 0; c < D / 16; c++) {
+              const int at = c0 + half * (D / 16) + c;
+              *reinterpret_cast<uint4*>(dst + (at / 8) * TC_TILE + sw128(row, at % 8)) = x[c];
+            }
         }
       }
       fence_async_proxy();
@@ -288,7 +290,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
           if (m == -INFINITY) {
             m = top;                                 // (a row's first keys: its sums are zero)
           } else if ((top - m) * c2 > 8.0f) {
-            alpha = ex2_approx((m - top) * c2);
+            alpha = ex2((m - top) * c2);
             l *= alpha;
             m = top;
           }
@@ -314,7 +316,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
           for (int x = 0; x < 32; x++) {
             const uint32_t* y = &v[x / 16][2 * (x % 16)];
             const float2 e = fma2(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), make_float2(c2, c2), make_float2(neg, neg));
-            const float2 pp = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+            const float2 pp = make_float2(ex2(e.x), ex2(e.y));
             sum[x & 1] = add2(sum[x & 1], pp);
             const __nv_bfloat162 hh = __floats2bfloat162_rn(pp.x, pp.y);
             p[x] = *reinterpret_cast<const uint32_t*>(&hh);
