@@ -11,6 +11,7 @@
 // lengths.  What a block finds for (a piece of) an item goes to the workspace.  The second launch makes the tokens' own parts,
 // which it does while the first still runs, waits for that, and joins all parts of a (token, head).
 #include "attention_prefix.cuh"
+#include "attention_prefix_own.cuh"
 #include "attention_prefix_tc.cuh"
 
 SGLC_DEFINE_ERROR_STRING()
@@ -615,5 +616,6 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   a.o_vec = ((uintptr_t)out & 15) == 0 && o_stride * (dtype == SGLC_F32 ? 4 : 2) % 16 == 0;
   const int code = a.tc ? (D == 64 ? launch_tc<64, 4>(a, stream) : launch_tc<128, 2>(a, stream)) : dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
   if (code) return code;
+  if (join_pays(a)) return D == 64 ? run_join<64>(a, max_own, stream) : run_join<128>(a, max_own, stream);
   return dtype == SGLC_F32 ? run_own<float>(a, max_own, stream) : run_own<__nv_bfloat16>(a, max_own, stream);
 }

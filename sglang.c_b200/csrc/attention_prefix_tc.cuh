@@ -231,34 +231,30 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       const int lim = valid ? visible(a, t, s.keys) : 0;
       // both groups are done with the item before (its products have been waited for): queries of this one
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      {
-        // (the same 128 rows for both groups: half of the columns each; all pieces asked for at once)
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)(s.hk * gq + n - (t - s.t0) * gq) * D;
-        const int c0 = pair ? 0 : w * (D / 16);
-        uint8_t* dst = sQ + (pair ? w * UNIT : 0);
+      // (all 256 threads, pieces of 16 bytes side by side: a thread a row took 12,000 cycles for 256 rows of 128; eight asked
+      // for at a time)
+      for (int x0 = threadIdx.x; x0 < (D / 8) << s.shift; x0 += 8 * 2 * TC_WG) {
+        uint4 x[8];
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          uint4 x[D / 16];
-#pragma unroll
-          for (int c = 0; c < D / 16; c++) {
-            x[c] = make_uint4(0u, 0u, 0u, 0u);
-            const __nv_bfloat16* from = src + (c0 + half * (D / 16) + c) * 8;
-            if (valid && (pair || half == 0)) {
-              if (a.q_vec) {
-                x[c] = *reinterpret_cast<const uint4*>(from);
-              } else {
-                const unsigned short* h = reinterpret_cast<const unsigned short*>(from);
-                x[c] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                                  h[6] | (uint32_t)h[7] << 16);
-              }
+        for (int u = 0; u < 8; u++) {
+          const int at = x0 + u * 2 * TC_WG, r = at / (D / 8), c = at % (D / 8);
+          x[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows) {
+            const int nr = s.row0 + r, tr = (unsigned)nr / (unsigned)gq;
+            const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(s.t0 + tr) * a.q_stride + (size_t)(s.hk * gq + nr - tr * gq) * D + c * 8;
+            if (a.q_vec) {
+              x[u] = *reinterpret_cast<const uint4*>(from);
+            } else {
+              const unsigned short* h = reinterpret_cast<const unsigned short*>(from);
+              x[u] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                                h[6] | (uint32_t)h[7] << 16);
             }
           }
-          if (pair || half == 0)
+        }
 #pragma unroll
-            for (int c = 0; c < D / 16; c++) {
-              const int at = c0 + half * (D / 16) + c;
-              *reinterpret_cast<uint4*>(dst + (at / 8) * TC_TILE + sw128(row, at % 8)) = x[c];
-            }
+        for (int u = 0; u < 8; u++) {
+          const int at = x0 + u * 2 * TC_WG, r = at / (D / 8), c = at % (D / 8);
+          if (r < 1 << s.shift) *reinterpret_cast<uint4*>(sQ + (r / TC_WG) * UNIT + (c / 8) * TC_TILE + sw128(r % TC_WG, c % 8)) = x[u];
         }
       }
       fence_async_proxy();
