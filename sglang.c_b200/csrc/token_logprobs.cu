@@ -3,10 +3,11 @@
 //   m = max l,  s = sum exp(l - m),  w = sum (l - m) exp(l - m):
 //   logprob(t) = (l_t - m) - log s,   entropy = log s - w / s,
 //   place(t) = how many tokens come before t: those of a larger logit, and of the same one with a smaller id.
-// The row is read once: a thread keeps (m, s, w) of the pieces it meets, scaled to its running maximum, and the place is a
-// count.  The best k come from the threads' maxima: with T the k-th largest of these, every entry above T lies with one of
-// the fewer than k threads whose maximum is above T, so only those threads' pieces (a few hundredths of the row, still in
-// L2) are looked at again; entries equal to T fill up from the smallest id.
+// The row is read once: a thread keeps (m, s, w) of the entries it meets, sixteen at a time, scaled to its running maximum,
+// and the place is a count of those few sixteens that reach the token's logit.  The best k come from the threads'
+// maxima: k groups of threads have a maximum of T or more for T the k-th largest of the groups', so the best k are T or more,
+// and they lie with the few threads whose own maximum is: only those threads' pieces (a tenth of the row, still in
+// L2) are looked at again.
 // Sums are 32-bit, a thread's over V / 256 entries and then pairwise.  The exponential is the special-function unit's
 // (2 ulp) of a difference taken exactly as it is rounded, so no logit is too large for it.
 #include "common.cuh"
@@ -36,6 +37,29 @@ struct Args {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two at a time, each rounded as one alone.
+#define SGLC_TWO(name, op)                                                                                                       \
+  __device__ __forceinline__ float2 name(float2 x, float2 y) {                                                                   \
+    unsigned long long r;                                                                                                        \
+    asm(op ".rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y))); \
+    return reinterpret_cast<float2&>(r);                                                                                         \
+  }
+SGLC_TWO(add2, "add")
+SGLC_TWO(mul2, "mul")
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(x)), "l"(reinterpret_cast<unsigned long long&>(y)),
+      "l"(reinterpret_cast<unsigned long long&>(z)));
+  return reinterpret_cast<float2&>(r);
+}
+
+// the largest of the warp (numbers; NaN is passed over)
+__device__ __forceinline__ float warp_maximum(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -73,22 +97,31 @@ __device__ __forceinline__ unsigned long long key_of(float v, int id) {
   return ((unsigned long long)ordered(v) << 32) | (unsigned)~id;      // (never 0: that is "no entry")
 }
 
-struct Sums { float m, s, w; };           // w in units of log 2
+// Maximum; how many entries are it; sum over the others; sum of (l - m) exp(l - m), in units of log 2.  The ones are kept apart
+// so that log(n + s) of a row with one likely token, log1p(s), has the digits of s and not what 1 + s leaves of them.
+struct Sums {
+  float m, n, s, w;
+  __device__ __forceinline__ void rescale(float top) {        // to a larger maximum
+    if (m > -INFINITY) {
+      const float d = (m - top) * LOG2E, f = ex2(d);
+      // (a factor of 0 drops the share whole: 0 * -inf would make NaN of it)
+      w = f > 0.0f ? f * fmaf(d, n + s, w) : s * 0.0f;
+      s = (n + s) * f;
+      n = 0.0f;
+    }
+    m = top;
+  }
+};
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.w + b.w};       // (both 0, or NaN)
-  // a share without any finite entry has s = w = 0 (or NaN): its reference is taken as m
-  const float da = a.m == -INFINITY ? 0.0f : (a.m - m) * LOG2E, db = b.m == -INFINITY ? 0.0f : (b.m - m) * LOG2E;
-  const float fa = ex2(da), fb = ex2(db);
-  // (a factor of 0 drops its share whole: 0 * -inf would make NaN of it)
-  const float wa = fa > 0.0f ? fa * fmaf(da, a.s, a.w) : a.s * 0.0f, wb = fb > 0.0f ? fb * fmaf(db, b.s, b.w) : b.s * 0.0f;
-  return {m, a.s * fa + b.s * fb, wa + wb};
+  if (a.m > b.m) b.rescale(a.m);
+  if (b.m > a.m) a.rescale(b.m);
+  return {a.m, a.n + b.n, a.s + b.s, a.w + b.w};
 }
 
 struct Shared {
   Sums warp_sums[WARPS];
   int warp_count[WARPS];
-  float best[THREADS];                    // the threads' maxima
+  float group[64];                        // maxima of groups of threads
   int chosen[THREADS];
   int n_chosen, n_above, n_out;
   float threshold;
@@ -111,6 +144,7 @@ struct Part {
   static constexpr int N = Vec<T>::N;
   __device__ int rounds() const { return (last - first + THREADS - 1) / THREADS; }
   __device__ int id_of(int piece) const { return head + piece * N; }
+  __device__ bool is_in(int piece) const { return piece < last; }
   __device__ bool take(int piece, float (&v)[N]) const {
     if (piece < last) {
       Vec<T>::take(row + id_of(piece), v);
@@ -157,56 +191,97 @@ token_logprobs_kernel(const Args a) {
   const float tv = asked ? ranked(tv_raw) : INFINITY;
   const bool counts = asked && a.place;
 
-  // ---- one pass: maximum, sums, count ----
-  Sums x = {-INFINITY, 0.0f, 0.0f};
+  // ---- one pass: maximum, sums, count; sixteen entries of a thread at a time ----
+  // The reference is the warp's: a thread's own would be moved by some thread of the warp at nearly every turn.
+  Sums x = {-INFINITY, 0.0f, 0.0f, 0.0f};
+  float best = -INFINITY;                 // this thread's maximum
   int count = 0;
-  auto visit = [&](const float* v, const int n, const int id0) {
-    float bm = v[0];
-#pragma unroll
-    for (int i = 1; i < n; i++) bm = fmaxf(bm, v[i]);
-    if (bm > x.m) {
-      if (x.m > -INFINITY) {
-        const float d = (x.m - bm) * LOG2E, f = ex2(d);
-        x.w = f > 0.0f ? f * fmaf(d, x.s, x.w) : x.s * 0.0f;
-        x.s *= f;
-      }
-      x.m = bm;
-    }
-    const float m = x.m == -INFINITY ? 0.0f : x.m;
-#pragma unroll
-    for (int i = 0; i < n; i++) {
-      const float d = (v[i] - m) * LOG2E, e = ex2(d);
-      x.s += e;
-      x.w = fmaf(fmaxf(d, -200.0f), e, x.w);      // (an entry at -inf: e = 0, and 0 times a bounded number)
-    }
-    if (counts && (bm >= tv || tv == -INFINITY)) {
-#pragma unroll
-      for (int i = 0; i < n; i++) {
-        const float y = ranked(v[i]);
-        count += y > tv || (y == tv && id0 + i < tok);
-      }
-    }
-  };
-  for (int q = p.first + tid; q < p.last; q += THREADS * DEEP) {
+  // entries of the token's logit count before it by their ids; of a piece of 16 bytes all ids are smaller or none is
+  // (the token's own piece is looked at once more below)
+  const float above = __uint_as_float(tv >= 0.0f ? __float_as_uint(tv) + 1u : __float_as_uint(tv) - 1u);       // the next larger
+  // (rounds are the warp's: a thread past the part's end reads -inf)
+  for (int q = p.first + tid; q - lane < p.last; q += THREADS * DEEP) {
     float v[DEEP][N];
-    bool in[DEEP];
 #pragma unroll
-    for (int u = 0; u < DEEP; u++) in[u] = p.take(q + u * THREADS, v[u]);
+    for (int u = 0; u < DEEP; u++) p.take(q + u * THREADS, v[u]);
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int u = 0; u < DEEP; u++)
-      if (in[u]) visit(v[u], N, p.id_of(q + u * THREADS));
+    for (int i = 0; i < 16; i++) top[i & 3] = fmaxf(top[i & 3], v[i / N][i % N]);
+    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    best = fmaxf(best, top[0]);
+    const float warp_top = warp_maximum(top[0]);
+    const bool reaches = warp_top >= x.m;              // (then some of these may be the maximum, and are counted)
+    if (warp_top > x.m) x.rescale(warp_top);
+    const float m = x.m == -INFINITY ? 0.0f : x.m;
+    float2 s = make_float2(0.0f, 0.0f), w = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float2 d = mul2(add2(make_float2(v[i / N][i % N], v[i / N][i % N + 1]), make_float2(-m, -m)), make_float2(LOG2E, LOG2E));
+      const float2 e = make_float2(ex2(d.x), ex2(d.y));
+      s = add2(s, e);
+      w = fma2(d, e, w);
+    }
+    if (reaches) {                                     // (few turns: the sum again, without what is counted)
+      s = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const float e = ex2((v[i / N][i % N] - m) * LOG2E);
+        if (e == 1.0f) x.n += 1.0f;
+        else s.x += e;
+      }
+    }
+    if (!(w.x + w.y == w.x + w.y)) {
+      // an entry at -inf, where the exponential is 0 and the product with it should be: once more, with a bound (or an entry
+      // that is no number, and remains it)
+      w = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const float d = (v[i / N][i % N] - m) * LOG2E;
+        w.x = fmaf(fmaxf(d, -200.0f), ex2(d), w.x);
+      }
+    }
+    x.s += s.x + s.y;
+    x.w += w.x + w.y;
+    if (counts && top[0] >= tv) {
+      if (tv > -INFINITY) {
+#pragma unroll
+        for (int u = 0; u < DEEP; u++) {
+          const float from = p.id_of(q + u * THREADS) + N <= tok ? tv : above;
+#pragma unroll
+          for (int i = 0; i < N; i++) count += v[u][i] >= from;
+        }
+      }
+    }
+    if (counts && tv == -INFINITY) {                   // (a token that is not allowed: NaN counts as it, too)
+#pragma unroll
+      for (int i = 0; i < 16; i++) count += p.is_in(q + i / N * THREADS) && (ranked(v[i / N][i % N]) > tv || p.id_of(q + i / N * THREADS) + i % N < tok);
+    }
+  }
+  auto place_of = [&](float y, int id) { count += ranked(y) > tv || (ranked(y) == tv && id < tok); };
+  if (counts && tv > -INFINITY && tid < N) {           // the token's own piece: equal logits of smaller ids
+    const int piece = (tok - p.head) / N, id = p.id_of(piece) + tid;
+    if (tok >= p.head && piece >= p.first && piece < p.last && id < tok) count += ranked(to_f32(p.row[id])) == tv;
   }
   const int my_loose = p.loose(tid);
-  if (my_loose >= 0) {
-    const float v[1] = {to_f32(p.row[my_loose])};
-    visit(v, 1, my_loose);
+  const float loose = my_loose >= 0 ? to_f32(p.row[my_loose]) : -INFINITY;
+  if (p.ends) {
+    const float warp_top = warp_maximum(loose);
+    if (warp_top > x.m) x.rescale(warp_top);
+    if (my_loose >= 0) {
+      const float d = (loose - (x.m == -INFINITY ? 0.0f : x.m)) * LOG2E, e = ex2(d);
+      if (e == 1.0f) x.n += 1.0f;
+      else x.s += e;
+      x.w = fmaf(fmaxf(d, -200.0f), e, x.w);
+      best = fmaxf(best, loose);
+      if (counts) place_of(loose, my_loose);
+    }
   }
-  const float best = ranked(x.m);
+  best = ranked(best);
 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const Sums y = {__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.s, o),
-                    __shfl_xor_sync(0xffffffffu, x.w, o)};
+    const Sums y = {__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.n, o),
+                    __shfl_xor_sync(0xffffffffu, x.s, o), __shfl_xor_sync(0xffffffffu, x.w, o)};
     x = join(x, y);
     count += __shfl_xor_sync(0xffffffffu, count, o);
   }
@@ -214,7 +289,6 @@ token_logprobs_kernel(const Args a) {
     sh.warp_sums[warp] = x;
     sh.warp_count[warp] = count;
   }
-  sh.best[tid] = best;
   if (tid == 0) {
     sh.n_chosen = 0;
     sh.n_above = 0;
@@ -231,17 +305,28 @@ token_logprobs_kernel(const Args a) {
   // ---- the block's best k ----
   const int k = a.k;
   if (k > 0) {
-    int rank = 0;
-    for (int u = 0; u < THREADS; u += 4) {
-      const float4 y = *reinterpret_cast<const float4*>(&sh.best[u]);
-      const float z[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) rank += z[i] > best || (z[i] == best && u + i < tid);
+    // A threshold that at least k entries reach: the k-th largest of the maxima of 32 (64) groups of threads.  About
+    // -32 ln(1 - k / 32) entries reach it (31 at k = 20), in as many threads at most, if large ones are anywhere.
+    const int of_group = k <= 32 ? 8 : 4;
+    float top = best;
+    for (int o = of_group / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane % of_group == 0) sh.group[tid / of_group] = top;
+    __syncthreads();
+    if (warp == 0) {
+      for (int half = 0; half < (k <= 32 ? 1 : 2); half++) {
+        const int me = lane + 32 * half;
+        const float mine = sh.group[me];
+        int rank = 0;
+        for (int u = 0; u < (k <= 32 ? 32 : 64); u++) rank += sh.group[u] > mine || (sh.group[u] == mine && u < me);
+        if (rank == k - 1) sh.threshold = mine;
+      }
     }
-    if (rank == k - 1) sh.threshold = best;
     __syncthreads();
     float T0 = sh.threshold;
-    if (best > T0) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = tid;
+    // the threads with entries at the threshold or above, and those entries; where these are too many (equal logits), or the
+    // threshold is -inf (few tokens allowed), only what is above it, and then equal ones from the smallest id on
+    bool ties = T0 > -INFINITY;
+    if (ties ? best >= T0 : best > T0) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = tid;
     __syncthreads();
     const int n_chosen = sh.n_chosen, rounds = p.rounds();
     // f(value, id) of every entry of the chosen threads
@@ -259,16 +344,23 @@ token_logprobs_kernel(const Args a) {
         if (id >= 0) f(ranked(to_f32(p.row[id])), id);
       }
     };
-    auto collect = [&](float above) {
+    auto collect = [&]() {
       again([&](float v, int id) {
-        if (v > above) {
+        if (ties ? v >= T0 : v > T0) {
           const int at = atomicAdd(&sh.n_above, 1);
           if (at < ROOM) sh.above[at] = key_of(v, id);
         }
       });
       __syncthreads();
     };
-    collect(T0);
+    collect();
+    if (ties && sh.n_above > ROOM) {
+      ties = false;
+      __syncthreads();
+      if (tid == 0) sh.n_above = 0;
+      __syncthreads();
+      collect();
+    }
     if (sh.n_above > ROOM) {
       // More entries above the threshold than there is room for (large logits at one stride): the k-th largest value
       // itself, bit by bit, by counting.  It becomes the threshold, so fewer than k entries are above it.
@@ -292,7 +384,7 @@ token_logprobs_kernel(const Args a) {
       __syncthreads();
       if (tid == 0) sh.n_above = 0;
       __syncthreads();
-      collect(T0);
+      collect();
     }
     const int n_above = sh.n_above;
     for (int c = tid; c < n_above; c += THREADS) {
@@ -336,14 +428,14 @@ token_logprobs_kernel(const Args a) {
         fill(v, in ? 1 : 0, from + tid);
       }
     };
-    fill_loose(0, p.head);
-    for (int i = 0; i < rounds && have < k; i++) {
+    if (!ties) fill_loose(0, p.head);
+    for (int i = 0; !ties && i < rounds && have < k; i++) {
       float v[N];
       const int q = p.first + tid + i * THREADS;
       const bool in = p.take(q, v);
       fill(v, in ? N : 0, p.id_of(q));
     }
-    fill_loose(p.tail, p.V);
+    if (!ties) fill_loose(p.tail, p.V);
     have = min(have, k);
     if (tid >= have && tid < k) sh.list[tid] = 0;           // a part of fewer than k entries
     __syncthreads();
@@ -358,9 +450,9 @@ token_logprobs_kernel(const Args a) {
       return at;
     };
     if (tid == 0) {
-      const float f[3] = {x.m, x.s, x.w};
+      const float f[4] = {x.m, x.n, x.s, x.w};
 #pragma unroll
-      for (int i = 0; i < 3; i++)
+      for (int i = 0; i < 4; i++)
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there(&sh.row_sums[share]) + 4 * i), "f"(f[i]) : "memory");
       asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(there(&sh.row_count[share])), "r"(count) : "memory");
     }
@@ -384,11 +476,12 @@ token_logprobs_kernel(const Args a) {
     __syncthreads();
   }
 
-  const bool none = x.s == 0.0f;                            // every entry at -inf (NaN is not 0)
-  const float log_s = logf(x.s);
+  const float total = x.n + x.s;
+  const bool none = total == 0.0f;                          // every entry at -inf (NaN is not 0)
+  const float log_s = x.n == 1.0f ? log1pf(x.s) : logf(total);
   if (tid == 0) {
     a.logprob[r] = !asked ? 0.0f : none ? -INFINITY : (tv_raw - x.m) - log_s;
-    if (a.entropy) a.entropy[r] = none ? 0.0f : log_s - LN2 * (x.w / x.s);
+    if (a.entropy) a.entropy[r] = none ? 0.0f : log_s - LN2 * (x.w / total);
     if (a.place) a.place[r] = asked ? count : -1;
   }
   if (tid < k) {
