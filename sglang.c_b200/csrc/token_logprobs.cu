@@ -6,8 +6,8 @@
 // The row is read once: a thread keeps (m, s, w) of the entries it meets, sixteen at a time, scaled to its running maximum,
 // and the place is a count of those few sixteens that reach the token's logit.  The best k come from the threads'
 // maxima: k groups of threads have a maximum of T or more for T the k-th largest of the groups', so the best k are T or more,
-// and they lie with the few threads whose own maximum is: only those threads' pieces (a tenth of the row, still in
-// L2) are looked at again.
+// and they lie in the few stretches of a thread's turns whose own maximum is: only those (a hundredth of the row,
+// still in L2) are looked at again.
 // Sums are 32-bit, a thread's over V / 256 entries and then pairwise.  The exponential is the special-function unit's
 // (2 ulp) of a difference taken exactly as it is rounded, so no logit is too large for it.
 #include "common.cuh"
@@ -17,8 +17,10 @@ SGLC_DEFINE_ERROR_STRING()
 namespace {
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
+constexpr int RESIDENT = 4;              // blocks a multiprocessor holds
 constexpr int MAX_TOP = 64;
 constexpr int ROOM = 1024;               // entries above the threshold that are sorted in shared memory
+constexpr int SEGMENTS = 8;              // stretches of a thread's turns whose maxima are kept
 constexpr int MAX_SHARES = 8;            // blocks of a row (one cluster)
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -66,15 +68,15 @@ __device__ __forceinline__ float warp_maximum(float x) {
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
-  __device__ static void take(const float* p, float (&v)[4]) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(p));
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  }
+  typedef float4 Raw;
+  __device__ static Raw none() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
+  __device__ static void open(const Raw& x, float (&v)[4]) { v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  __device__ static void take(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+  typedef uint4 Raw;
+  __device__ static Raw none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }       // (-inf)
+  __device__ static void open(const Raw& x, float (&v)[8]) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -122,7 +124,8 @@ struct Shared {
   Sums warp_sums[WARPS];
   int warp_count[WARPS];
   float group[64];                        // maxima of groups of threads
-  int chosen[THREADS];
+  float seg[SEGMENTS][THREADS];           // a thread's maxima of stretches of its turns
+  int chosen[SEGMENTS * THREADS];         // (stretch, thread)
   int n_chosen, n_above, n_out;
   float threshold;
   unsigned long long above[ROOM];
@@ -145,14 +148,12 @@ struct Part {
   __device__ int rounds() const { return (last - first + THREADS - 1) / THREADS; }
   __device__ int id_of(int piece) const { return head + piece * N; }
   __device__ bool is_in(int piece) const { return piece < last; }
+  __device__ typename Vec<T>::Raw raw(int piece) const {       // (-inf where the part ends)
+    return piece < last ? __ldg(reinterpret_cast<const typename Vec<T>::Raw*>(row + id_of(piece))) : Vec<T>::none();
+  }
   __device__ bool take(int piece, float (&v)[N]) const {
-    if (piece < last) {
-      Vec<T>::take(row + id_of(piece), v);
-      return true;
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = -INFINITY;
-    return false;
+    Vec<T>::open(raw(piece), v);
+    return piece < last;
   }
   // the loose entry of thread `t`, or -1
   __device__ int loose(int t) const {
@@ -164,30 +165,38 @@ struct Part {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, RESIDENT)
 token_logprobs_kernel(const Args a) {
   constexpr int N = Vec<T>::N;
   constexpr int DEEP = 16 / N;            // pieces in flight a thread
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int share = blockIdx.z, shares = gridDim.z;
-  const long long r = blockIdx.x;
   // (that this block has begun, for the others of the row's cluster, which store into block 0's shared memory below)
   if (shares > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_launch_dependents();
-  Part<T> p;
-  p.row = reinterpret_cast<const T*>(a.logits) + r * a.ld;
-  p.V = a.V;
-  p.head = min(a.V, (int)((16 - ((uintptr_t)p.row & 15)) & 15) / (int)sizeof(T));
-  const int pieces = (a.V - p.head) / N;
-  p.tail = p.head + pieces * N;
-  p.first = (int)((long long)pieces * share / shares);
-  p.last = (int)((long long)pieces * (share + 1) / shares);
-  p.ends = share == 0;
+  auto part_of = [&](long long row) {
+    Part<T> x;
+    x.row = reinterpret_cast<const T*>(a.logits) + row * a.ld;
+    x.V = a.V;
+    x.head = min(a.V, (int)((16 - ((uintptr_t)x.row & 15)) & 15) / (int)sizeof(T));
+    const int pieces = (a.V - x.head) / N;
+    x.tail = x.head + pieces * N;
+    x.first = (int)((long long)pieces * share / shares);
+    x.last = (int)((long long)pieces * (share + 1) / shares);
+    x.ends = share == 0;
+    return x;
+  };
+  // (the first pieces are asked for ahead of the chain row -> token -> its logit)
+  typename Vec<T>::Raw next[DEEP];
+  const long long r = blockIdx.x;
+  const Part<T> p = part_of(r);
+#pragma unroll
+  for (int u = 0; u < DEEP; u++) next[u] = p.raw(p.first + tid + u * THREADS);
   const int tok = a.tokens ? a.tokens[r] : -1;
+  const float tv_raw = tok >= 0 && tok < a.V ? to_f32(p.row[tok]) : 0.0f;
   const bool asked = tok >= 0 && tok < a.V;
-  const float tv_raw = asked ? to_f32(p.row[tok]) : 0.0f;
   const float tv = asked ? ranked(tv_raw) : INFINITY;
   const bool counts = asked && a.place;
 
@@ -200,15 +209,26 @@ token_logprobs_kernel(const Args a) {
   // (the token's own piece is looked at once more below)
   const float above = __uint_as_float(tv >= 0.0f ? __float_as_uint(tv) + 1u : __float_as_uint(tv) - 1u);       // the next larger
   // (rounds are the warp's: a thread past the part's end reads -inf)
-  for (int q = p.first + tid; q - lane < p.last; q += THREADS * DEEP) {
+  const int turns = (p.last - p.first + THREADS * DEEP - 1) / (THREADS * DEEP), stretch = (turns + SEGMENTS - 1) / SEGMENTS;
+  float seg_best = -INFINITY;
+  int seg = 0, seg_turn = 0;
+  for (int q = p.first + tid; q - tid < p.last; q += THREADS * DEEP) {
     float v[DEEP][N];
 #pragma unroll
-    for (int u = 0; u < DEEP; u++) p.take(q + u * THREADS, v[u]);
+    for (int u = 0; u < DEEP; u++) Vec<T>::open(next[u], v[u]);
+#pragma unroll
+    for (int u = 0; u < DEEP; u++) next[u] = p.raw(q + (DEEP + u) * THREADS);
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < 16; i++) top[i & 3] = fmaxf(top[i & 3], v[i / N][i % N]);
     top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    best = fmaxf(best, top[0]);
+    seg_best = fmaxf(seg_best, top[0]);
+    if (++seg_turn == stretch) {
+      sh.seg[seg++][tid] = seg_best;
+      best = fmaxf(best, seg_best);
+      seg_best = -INFINITY;
+      seg_turn = 0;
+    }
     const float warp_top = warp_maximum(top[0]);
     const bool reaches = warp_top >= x.m;              // (then some of these may be the maximum, and are counted)
     if (warp_top > x.m) x.rescale(warp_top);
@@ -257,13 +277,19 @@ token_logprobs_kernel(const Args a) {
       for (int i = 0; i < 16; i++) count += p.is_in(q + i / N * THREADS) && (ranked(v[i / N][i % N]) > tv || p.id_of(q + i / N * THREADS) + i % N < tok);
     }
   }
-  auto place_of = [&](float y, int id) { count += ranked(y) > tv || (ranked(y) == tv && id < tok); };
-  if (counts && tv > -INFINITY && tid < N) {           // the token's own piece: equal logits of smaller ids
-    const int piece = (tok - p.head) / N, id = p.id_of(piece) + tid;
-    if (tok >= p.head && piece >= p.first && piece < p.last && id < tok) count += ranked(to_f32(p.row[id])) == tv;
+  if (seg_turn > 0) {
+    sh.seg[seg++][tid] = seg_best;
+    best = fmaxf(best, seg_best);
   }
+  auto place_of = [&](float y, int id) { count += ranked(y) > tv || (ranked(y) == tv && id < tok); };
+  // single entries that are looked at below: before and behind the pieces; of the token's own piece
   const int my_loose = p.loose(tid);
   const float loose = my_loose >= 0 ? to_f32(p.row[my_loose]) : -INFINITY;
+  const int own_piece = asked && tok >= p.head ? (tok - p.head) / N : -1, own_id = p.id_of(own_piece) + tid;
+  const bool owns = counts && tid < N && own_piece >= p.first && own_piece < p.last && own_id < tok;
+  const float own = owns ? ranked(to_f32(p.row[own_id])) : 0.0f;
+
+  if (owns && tv > -INFINITY) count += own == tv;       // the token's own piece: equal logits of smaller ids
   if (p.ends) {
     const float warp_top = warp_maximum(loose);
     if (warp_top > x.m) x.rescale(warp_top);
@@ -278,71 +304,102 @@ token_logprobs_kernel(const Args a) {
   }
   best = ranked(best);
 
+  // ---- the block's sums and count (warp 0), and a threshold for its best k ----
+  // At least k entries reach the threshold: it is the k-th largest of the maxima of 32 (64) groups of threads.  About
+  // -32 ln(1 - k / 32) entries do (31 at k = 20), and so many threads at most have them.
+  const int k = a.k, groups = k <= 32 ? 32 : 64, of_group = THREADS / groups;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums y = {__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.n, o),
-                    __shfl_xor_sync(0xffffffffu, x.s, o), __shfl_xor_sync(0xffffffffu, x.w, o)};
-    x = join(x, y);
-    count += __shfl_xor_sync(0xffffffffu, count, o);
+  for (int o = 16; o > 0; o >>= 1) {                 // (the warp's lanes have one reference)
+    x.n += __shfl_xor_sync(0xffffffffu, x.n, o);
+    x.s += __shfl_xor_sync(0xffffffffu, x.s, o);
+    x.w += __shfl_xor_sync(0xffffffffu, x.w, o);
   }
+  count = __reduce_add_sync(0xffffffffu, count);
   if (lane == 0) {
     sh.warp_sums[warp] = x;
     sh.warp_count[warp] = count;
+  }
+  if (k > 0) {
+    float top = best;
+    for (int o = of_group / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane % of_group == 0) sh.group[tid / of_group] = top;
   }
   if (tid == 0) {
     sh.n_chosen = 0;
     sh.n_above = 0;
   }
   __syncthreads();
-  x = sh.warp_sums[0];
-  count = sh.warp_count[0];
+  if (warp == 0) {
+    x = lane < WARPS ? sh.warp_sums[lane] : Sums{-INFINITY, 0.0f, 0.0f, 0.0f};
+    count = __reduce_add_sync(0xffffffffu, lane < WARPS ? sh.warp_count[lane] : 0);
+    const float top = warp_maximum(x.m);
+    if (top > x.m) x.rescale(top);
 #pragma unroll
-  for (int w = 1; w < WARPS; w++) {
-    x = join(x, sh.warp_sums[w]);
-    count += sh.warp_count[w];
+    for (int o = WARPS / 2; o > 0; o >>= 1) {
+      x.n += __shfl_xor_sync(0xffffffffu, x.n, o);
+      x.s += __shfl_xor_sync(0xffffffffu, x.s, o);
+      x.w += __shfl_xor_sync(0xffffffffu, x.w, o);
+    }
+    for (int me = lane; k > 0 && me < groups; me += 32) {
+      const float mine = sh.group[me];
+      int rank = 0;
+      for (int u = 0; u < groups; u++) rank += sh.group[u] > mine || (sh.group[u] == mine && u < me);
+      if (rank == k - 1) sh.threshold = mine;
+    }
+    if (lane == 0 && shares == 1) sh.row_sums[0] = x;
   }
+  // what is known of the row, and of token `id` with logit v at place i of the order
+  auto give_row = [&](const Sums& x, int count) {
+    const float total = x.n + x.s;
+    const bool none = total == 0.0f;                        // every entry at -inf (NaN is not 0)
+    const float log_s = x.n == 1.0f ? log1pf(x.s) : logf(total);
+    a.logprob[r] = !asked ? 0.0f : none ? -INFINITY : (tv_raw - x.m) - log_s;
+    if (a.entropy) a.entropy[r] = none ? 0.0f : log_s - LN2 * (x.w / total);
+    if (a.place) a.place[r] = asked ? count : -1;
+  };
+  auto give_top = [&](const Sums& x, unsigned long long key, int i) {
+    const float total = x.n + x.s, log_s = x.n == 1.0f ? log1pf(x.s) : logf(total), v = unordered((unsigned)(key >> 32));
+    a.top_ids[r * a.top_ld + i] = (int)~(unsigned)key;
+    a.top_logprobs[r * a.top_ld + i] = total == 0.0f ? -INFINITY : (v - x.m) - log_s;
+  };
 
   // ---- the block's best k ----
-  const int k = a.k;
   if (k > 0) {
-    // A threshold that at least k entries reach: the k-th largest of the maxima of 32 (64) groups of threads.  About
-    // -32 ln(1 - k / 32) entries reach it (31 at k = 20), in as many threads at most, if large ones are anywhere.
-    const int of_group = k <= 32 ? 8 : 4;
-    float top = best;
-    for (int o = of_group / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane % of_group == 0) sh.group[tid / of_group] = top;
-    __syncthreads();
-    if (warp == 0) {
-      for (int half = 0; half < (k <= 32 ? 1 : 2); half++) {
-        const int me = lane + 32 * half;
-        const float mine = sh.group[me];
-        int rank = 0;
-        for (int u = 0; u < (k <= 32 ? 32 : 64); u++) rank += sh.group[u] > mine || (sh.group[u] == mine && u < me);
-        if (rank == k - 1) sh.threshold = mine;
-      }
-    }
     __syncthreads();
     float T0 = sh.threshold;
-    // the threads with entries at the threshold or above, and those entries; where these are too many (equal logits), or the
+    // the stretches with entries at the threshold or above, and those entries; where these are too many (equal logits), or the
     // threshold is -inf (few tokens allowed), only what is above it, and then equal ones from the smallest id on
     bool ties = T0 > -INFINITY;
-    if (ties ? best >= T0 : best > T0) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = tid;
+    if (best >= T0)
+      for (int i = 0; i < seg; i++)
+        if (ties ? ranked(sh.seg[i][tid]) >= T0 : ranked(sh.seg[i][tid]) > T0) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = i * THREADS + tid;
     __syncthreads();
-    const int n_chosen = sh.n_chosen, rounds = p.rounds();
-    // f(value, id) of every entry of the chosen threads
+    const int rounds = p.rounds(), of_seg = stretch * DEEP, items = sh.n_chosen * of_seg;
+    // f(value, id) of every entry of the chosen stretches, and of those before and behind the pieces
     auto again = [&](auto&& f) {
-      for (int c = tid; c < n_chosen * rounds; c += THREADS) {
-        const int t = sh.chosen[c / rounds], q = p.first + t + c % rounds * THREADS;
-        float v[N];
-        if (p.take(q, v)) {
+      for (int c0 = tid; c0 < items; c0 += 2 * THREADS) {
+        typename Vec<T>::Raw x[2];
+        int q[2];
 #pragma unroll
-          for (int i = 0; i < N; i++) f(ranked(v[i]), p.id_of(q) + i);
+        for (int u = 0; u < 2; u++) {                 // (two on their way at a time)
+          const int c = c0 + u * THREADS, which = (unsigned)c / (unsigned)of_seg;
+          q[u] = p.last;
+          if (c < items) {
+            const int st = sh.chosen[which];
+            q[u] = p.first + st % THREADS + (st / THREADS * of_seg + c - which * of_seg) * THREADS;
+          }
+          x[u] = p.raw(q[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          float v[N];
+          Vec<T>::open(x[u], v);
+          if (p.is_in(q[u]))
+#pragma unroll
+            for (int i = 0; i < N; i++) f(ranked(v[i]), p.id_of(q[u]) + i);
         }
       }
-      if (tid < n_chosen) {
-        const int id = p.loose(sh.chosen[tid]);
-        if (id >= 0) f(ranked(to_f32(p.row[id])), id);
-      }
+      if (my_loose >= 0) f(ranked(loose), my_loose);
     };
     auto collect = [&]() {
       again([&](float v, int id) {
@@ -387,6 +444,17 @@ token_logprobs_kernel(const Args a) {
       collect();
     }
     const int n_above = sh.n_above;
+    if (shares == 1 && ties) {                              // the usual end: whoever ranks an entry gives it out
+      x = sh.row_sums[0];
+      if (tid == 0) give_row(x, count);
+      for (int c = tid; c < n_above; c += THREADS) {
+        const unsigned long long key = sh.above[c];
+        int before = 0;
+        for (int u = 0; u < n_above; u++) before += sh.above[u] > key;
+        if (before < k) give_top(x, key, before);
+      }
+      return;
+    }
     for (int c = tid; c < n_above; c += THREADS) {
       const unsigned long long key = sh.above[c];
       int before = 0;
@@ -476,21 +544,9 @@ token_logprobs_kernel(const Args a) {
     __syncthreads();
   }
 
-  const float total = x.n + x.s;
-  const bool none = total == 0.0f;                          // every entry at -inf (NaN is not 0)
-  const float log_s = x.n == 1.0f ? log1pf(x.s) : logf(total);
-  if (tid == 0) {
-    a.logprob[r] = !asked ? 0.0f : none ? -INFINITY : (tv_raw - x.m) - log_s;
-    if (a.entropy) a.entropy[r] = none ? 0.0f : log_s - LN2 * (x.w / total);
-    if (a.place) a.place[r] = asked ? count : -1;
-  }
-  if (tid < k) {
-    const unsigned long long key = sh.list[tid];
-    const int id = (int)~(unsigned)key;
-    a.top_ids[r * a.top_ld + tid] = id;
-    const float v = unordered((unsigned)(key >> 32));
-    a.top_logprobs[r * a.top_ld + tid] = none ? -INFINITY : (v - x.m) - log_s;
-  }
+  if (shares == 1 && k > 0) x = sh.row_sums[0];
+  if (tid == 0) give_row(x, count);
+  if (tid < k) give_top(x, sh.list[tid], tid);
 }
 
 // Blocks of a row.  Few rows are dealt to several blocks each, down to 512 pieces of 16 bytes a block.
