@@ -316,12 +316,39 @@ def kv_write(k_src, v_src, cache, slots, n_kv_heads, head_dim):
     _check(lib, code, "kv_write")
 
 
-def _on_current_device(what, *tensors):
-    """The kernels run on the current device's stream: every tensor has to lie there."""
-    here = torch.cuda.current_device()
+_INT, _FLOAT = torch.int32, torch.float32
+_functions = {}              # (library, launcher) -> the ctypes function with its argument types declared
+
+
+def _function(library, name, types, result=ctypes.c_int):
+    """A launcher whose arguments are converted by ctypes itself from plain integers and floats (declared types cost a call
+    a twentieth of a microsecond an argument, objects made for it a quarter; a step's smallest calls are bound by that).
+    types: "p" pointer, "i" int, "q" long long, "f" float, one letter an argument."""
+    lib = build.load(library)
+    hit = _functions.get((library, name))
+    if hit is None or hit[0] is not lib:
+        fn = getattr(lib, name)
+        fn.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}[t] for t in types]
+        fn.restype = result
+        hit = _functions[(library, name)] = (lib, fn)
+    return hit
+
+
+def _stream_here(device):
+    """_stream() for a call on the current device, number `device`."""
+    if _PROFILE is not None or _PINNED_STREAM is not None:
+        return _stream()
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _here(what, *tensors):
+    """The current device's number.  The kernels run on its stream: every tensor has to lie there."""
+    here = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
+            _need_cuda(t)
             raise KernelError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{here}")
+    return here
 
 
 STEP_TABLES_REQUESTS = 16384     # requests step_tables takes (step_tables.cu: MAX_REQUESTS)
@@ -339,19 +366,20 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
     All or nothing: where the pages are too few (status 1), a row too short (2), the tokens more than the arrays hold (4)
     or a length is out of range (8; sums of these), only status is written.  All arrays int32.  new_len and left are
     not kv_len and n_free (every block reads those)."""
-    arrays = dict(q_len=q_len, kv_len=kv_len, free_pages=free_pages, n_free=n_free, q_start=q_start, new_len=new_len,
-                  token_req=token_req, positions=positions, slots=slots, left=left, status=status)
-    _need_cuda(block_table, *arrays.values())
-    _on_current_device("step_tables", block_table, *arrays.values())
-    for nm, t in arrays.items():
-        _i32(t, f"step_tables: {nm}")
-    R = q_len.numel()
+    arrays = (q_len, kv_len, free_pages, n_free, q_start, new_len, token_req, positions, slots, left, status)
+    here = _here("step_tables", block_table, *arrays)
+    for t in arrays:
+        if t.dtype is not _INT or not t.is_contiguous():
+            names = ("q_len", "kv_len", "free_pages", "n_free", "q_start", "new_len", "token_req", "positions", "slots", "left", "status")
+            _i32(t, f"step_tables: {next(n for n, x in zip(names, arrays) if x is t)}")
+    R, T = q_len.numel(), token_req.numel()
     if R > STEP_TABLES_REQUESTS:
         raise KernelError(f"step_tables: {R} requests; at most {STEP_TABLES_REQUESTS}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < R \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1) or block_table.stride(0) < block_table.shape[1]:
+    if block_table.dtype is not _INT or block_table.dim() != 2:
         raise KernelError(f"step_tables: block_table must be int32 rows for {R} requests")
-    T = token_req.numel()
+    (rows, width), (pitch, column) = block_table.shape, block_table.stride()
+    if rows < R or (width > 1 and column != 1) or pitch < width:
+        raise KernelError(f"step_tables: block_table must be int32 rows for {R} requests")
     if kv_len.numel() < R or new_len.numel() < R or q_start.numel() < R + 1 or positions.numel() != T or slots.numel() != T:
         raise KernelError("step_tables: kv_len and new_len have an entry a request, q_start one more, and token_req, positions "
                           "and slots one length")
@@ -359,14 +387,14 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
         raise KernelError("step_tables: n_free, left and status are one word each")
     if int(page_size) != page_size or not 0 < page_size <= 1 << 20:
         raise KernelError(f"step_tables: page size {page_size}")
-    if left.data_ptr() == n_free.data_ptr() or (R and new_len.data_ptr() == kv_len.data_ptr()):
+    lens, after, n, n_after = kv_len.data_ptr(), new_len.data_ptr(), n_free.data_ptr(), left.data_ptr()
+    if n_after == n or (R and after == lens):
         raise KernelError("step_tables: new_len and left must be other memory than kv_len and n_free")
-    lib = build.load("step_tables")
-    code = lib.sglc_step_tables(_ptr(q_len), _ptr(kv_len), _ptr(free_pages), free_pages.numel(), _ptr(n_free),
-                                _ptr(block_table), ctypes.c_longlong(block_table.stride(0)), block_table.shape[1], R,
-                                int(page_size), _ptr(q_start), _ptr(new_len), _ptr(token_req), _ptr(positions), _ptr(slots), T,
-                                _ptr(left), _ptr(status), _stream())
-    _check(lib, code, f"step_tables ({R} requests)")
+    lib, fn = _function("step_tables", "sglc_step_tables", "pppippqiiippppp" "ipp" "p")
+    code = fn(q_len.data_ptr(), lens, free_pages.data_ptr(), free_pages.numel(), n, block_table.data_ptr(), pitch, width, R,
+              int(page_size), q_start.data_ptr(), after, token_req.data_ptr(), positions.data_ptr(), slots.data_ptr(), T, n_after,
+              status.data_ptr(), _stream_here(here))
+    _check(lib, code, "step_tables")
 
 
 def _gate_args(gate, T, n_heads, width, what):
@@ -760,16 +788,24 @@ def attention_latent_decode(q, cache, block_table, token_req, positions, out, n_
 PREFIX_GROUPS = 256       # groups attention_prefix takes (attention_prefix.cuh: MAX_GROUPS)
 
 
+_prefix_sizes = {}        # sizes and device -> floats of workspace
+
+
 def attention_prefix_workspace(n_tokens, n_groups, n_heads, n_kv_heads, dim, dtype):
     """float32 elements of workspace that attention_prefix takes for such a call on the current device."""
-    lib = build.load("attention_prefix")
-    lib.sglc_attention_prefix_workspace.restype = ctypes.c_longlong
-    if dtype not in _DT:
-        raise KernelError(f"attention_prefix: dtype {dtype} is not handled (float32 or bfloat16)")
-    n = lib.sglc_attention_prefix_workspace(int(n_tokens), int(n_groups), int(n_heads), int(n_kv_heads), int(dim), _DT[dtype])
-    if n < 0:
-        raise KernelError(f"attention_prefix: {n_heads} heads over {n_kv_heads} of size {dim}, {n_groups} groups: heads in whole "
-                          f"groups, sizes that are multiples of 8 up to 256, at most {PREFIX_GROUPS} groups of requests")
+    key = (n_tokens, n_groups, n_heads, n_kv_heads, dim, dtype, torch._C._cuda_getDevice())
+    n = _prefix_sizes.get(key)
+    if n is None:
+        if dtype not in _DT:
+            raise KernelError(f"attention_prefix: dtype {dtype} is not handled (float32 or bfloat16)")
+        _, fn = _function("attention_prefix", "sglc_attention_prefix_workspace", "iiiiii", ctypes.c_longlong)
+        n = fn(int(n_tokens), int(n_groups), int(n_heads), int(n_kv_heads), int(dim), _DT[dtype])
+        if n < 0:
+            raise KernelError(f"attention_prefix: {n_heads} heads over {n_kv_heads} of size {dim}, {n_groups} groups: heads in "
+                              f"whole groups, sizes that are multiples of 8 up to 256, at most {PREFIX_GROUPS} groups of requests")
+        if len(_prefix_sizes) >= 4096:
+            _prefix_sizes.clear()
+        _prefix_sizes[key] = n
     return n
 
 
@@ -789,44 +825,46 @@ def attention_prefix(q, cache, block_table, token_req, positions, group_start, s
     sizes the launch.  workspace: float32, attention_prefix_workspace() elements or more, used by this call alone
     until it is done (None: taken from torch's allocator).  An index out of range (a request, a page, a position beyond the
     table's row) is not followed and sets the error word (tc_error_flag)."""
-    _need_cuda(q, cache, block_table, token_req, positions, group_start, shared_len, out, workspace)
-    _on_current_device("attention_prefix", q, cache, block_table, token_req, positions, group_start, shared_len, out, workspace)
+    here = _here("attention_prefix", q, cache, block_table, token_req, positions, group_start, shared_len, out, workspace)
     for t, nm in ((token_req, "token_req"), (positions, "positions"), (group_start, "group_start"), (shared_len, "shared_len")):
-        if t is not None:
+        if t is not None and (t.dtype is not _INT or not t.is_contiguous()):
             _i32(t, f"attention_prefix: {nm}")
     if cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous():
         raise KernelError("attention_prefix: the cache is [n_pages, 2, n_kv_heads, page_size, head_dim], contiguous")
     n_pages, _, Hkv, page_size, D = cache.shape
-    T, G = q.shape[0], shared_len.numel()
-    if q.dim() != 2 or out.dim() != 2 or q.shape[1] != n_heads * D or out.shape[1] != n_heads * D or out.shape[0] < T \
-            or q.stride(1) != 1 or out.stride(1) != 1:
+    G, dtype = shared_len.numel(), cache.dtype
+    if q.dim() != 2 or out.dim() != 2:
         raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
-    if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+    (T, q_width), (q_pitch, q_column), (rows, width), (pitch, column) = q.shape, q.stride(), out.shape, out.stride()
+    if q_width != n_heads * D or width != q_width or rows < T or q_column != 1 or column != 1:
+        raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
+    if rows > 1 and pitch < width:
         raise KernelError("attention_prefix: rows of out overlap")
-    if q.dtype != cache.dtype or out.dtype != cache.dtype:
+    if q.dtype is not dtype or out.dtype is not dtype:
         raise KernelError("attention_prefix: queries, cache and output must have one dtype")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype is not _INT or block_table.dim() != 2:
+        raise KernelError("attention_prefix: block_table must be int32 rows")
+    (n_req, n_blocks), (bt_pitch, bt_column) = block_table.shape, block_table.stride()
+    if n_blocks > 1 and bt_column != 1:
         raise KernelError("attention_prefix: block_table must be int32 rows")
     if positions.numel() < T or (token_req is not None and token_req.numel() < T) or group_start.numel() != G + 1:
         raise KernelError("attention_prefix: positions and token_req have an entry a token, group_start one more than shared_len")
     if not (0.0 < scale < float("inf")):
         raise KernelError(f"attention_prefix: scale {scale} must be positive")
-    if cache.data_ptr() % 16:
+    pages = cache.data_ptr()
+    if pages % 16:
         raise KernelError("attention_prefix: the cache must begin on 16 bytes")
-    need = attention_prefix_workspace(T, G, n_heads, Hkv, D, cache.dtype)
+    need = attention_prefix_workspace(T, G, n_heads, Hkv, D, dtype)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.float32, device=q.device)
-    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.numel() < need \
-            or workspace.data_ptr() % 16:
+        workspace = torch.empty(need, dtype=_FLOAT, device=q.device)
+    elif workspace.dtype is not _FLOAT or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16:
         raise KernelError(f"attention_prefix: the workspace must be {need} float32 elements or more, contiguous, on 16 bytes")
-    lib = build.load("attention_prefix")
-    code = lib.sglc_attention_prefix(
-        _ptr(q), ctypes.c_longlong(q.stride(0)), _ptr(cache), _ptr(block_table), ctypes.c_longlong(block_table.stride(0)),
-        block_table.shape[1], block_table.shape[0], _ptr(token_req), _ptr(positions), _ptr(group_start), _ptr(shared_len), G,
-        _ptr(out), ctypes.c_longlong(out.stride(0)), T, n_heads, Hkv, D, page_size, n_pages, ctypes.c_float(scale),
-        max(0, int(max_own)), _ptr(workspace), ctypes.c_longlong(workspace.numel()), _dt(q, "attention_prefix"),
-        _ptr(tc_error_flag(q.device)), _stream())
-    _check(lib, code, f"attention_prefix (head_dim {D})", n_kernels=2)
+    lib, fn = _function("attention_prefix", "sglc_attention_prefix", "pqppqi" "ippppipq" "iiiiiifi" "pqipp")
+    code = fn(q.data_ptr(), q_pitch, pages, block_table.data_ptr(), bt_pitch, n_blocks, n_req,
+              None if token_req is None else token_req.data_ptr(), positions.data_ptr(), group_start.data_ptr(), shared_len.data_ptr(),
+              G, out.data_ptr(), pitch, T, n_heads, Hkv, D, page_size, n_pages, scale, max(0, int(max_own)), workspace.data_ptr(),
+              workspace.numel(), _DT[dtype], tc_error_flag(q.device).data_ptr(), _stream_here(here))
+    _check(lib, code, "attention_prefix", n_kernels=2)
 
 
 # ---------------------------------------------------------------------------
@@ -911,35 +949,40 @@ def token_logprobs(logits, tokens, logprob, entropy=None, place=None, top_ids=No
     A token outside 0..V-1 (say -1) asks for nothing: logprob 0, place -1.  tokens None: no row asks.  A logit
     of -inf is a token that is not allowed; a row without any allowed one has log-probabilities -inf and entropy 0.  A
     row with a logit that is NaN or +inf has NaN for both; in the order of choice NaN counts as -inf."""
-    _need_cuda(logits, tokens, logprob, entropy, place, top_ids, top_logprobs)
-    _on_current_device("token_logprobs", logits, tokens, logprob, entropy, place, top_ids, top_logprobs)
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    here = _here("token_logprobs", logits, tokens, logprob, entropy, place, top_ids, top_logprobs)
+    if logits.dim() != 2:
         raise KernelError("token_logprobs: logits must be rows of a vocabulary")
-    n, V = logits.shape
-    for t, nm, dt in ((tokens, "tokens", torch.int32), (logprob, "logprob", torch.float32), (entropy, "entropy", torch.float32),
-                      (place, "place", torch.int32)):
+    (n, V), (pitch, column) = logits.shape, logits.stride()
+    if V < 1 or (V > 1 and column != 1):
+        raise KernelError("token_logprobs: logits must be rows of a vocabulary")
+    for t, dt, nm in ((tokens, _INT, "tokens"), (logprob, _FLOAT, "logprob"), (entropy, _FLOAT, "entropy"), (place, _INT, "place")):
         if t is None and nm != "logprob":
             continue
-        if t.dtype != dt or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not dt or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
             raise KernelError(f"token_logprobs: {nm} must be a contiguous {dt} vector of an entry a row ({n})")
     if (top_ids is None) != (top_logprobs is None):
         raise KernelError("token_logprobs: top_ids and top_logprobs come together")
-    k = 0
+    k = top_pitch = 0
+    ids = best = None
     if top_ids is not None:
         k = top_ids.shape[1] if top_ids.dim() == 2 else -1
-        if k < 0 or tuple(top_ids.shape) != (n, k) or tuple(top_logprobs.shape) != (n, k) or top_ids.dtype != torch.int32 \
-                or top_logprobs.dtype != torch.float32:
+        if k < 0 or top_ids.shape != (n, k) or top_logprobs.shape != (n, k) or top_ids.dtype is not _INT \
+                or top_logprobs.dtype is not _FLOAT:
             raise KernelError("token_logprobs: top_ids must be int32 and top_logprobs float32, [rows, k] both")
         if k > min(V, TOP_TOKENS):
             raise KernelError(f"token_logprobs: {k} alternatives of {V} tokens; at most {TOP_TOKENS}")
-        if k > 1 and (top_ids.stride(1) != 1 or top_logprobs.stride(1) != 1) \
-                or n > 1 and k and top_ids.stride(0) != top_logprobs.stride(0):
-            raise KernelError("token_logprobs: top_ids and top_logprobs must be rows of one stride")
-    lib = build.load("token_logprobs")
-    code = lib.sglc_token_logprobs(_ptr(logits), ctypes.c_longlong(logits.stride(0)), _dt(logits, "token_logprobs"), n, V,
-                                   _ptr(tokens), _ptr(logprob), _ptr(entropy), _ptr(place), k, _ptr(top_ids), _ptr(top_logprobs),
-                                   ctypes.c_longlong(top_ids.stride(0) if k else 0), _stream())
-    _check(lib, code, f"token_logprobs (vocabulary {V})")
+        if k:
+            (top_pitch, top_column), (other, other_column) = top_ids.stride(), top_logprobs.stride()
+            if k > 1 and (top_column != 1 or other_column != 1) or n > 1 and top_pitch != other:
+                raise KernelError("token_logprobs: top_ids and top_logprobs must be rows of one stride")
+            if n > 1 and top_pitch < k:
+                raise KernelError("token_logprobs: rows of top_ids overlap")
+            ids, best = top_ids.data_ptr(), top_logprobs.data_ptr()
+    lib, fn = _function("token_logprobs", "sglc_token_logprobs", "pqiiipppp" "ippqp")
+    code = fn(logits.data_ptr(), pitch, _dt(logits, "token_logprobs"), n, V, None if tokens is None else tokens.data_ptr(),
+              logprob.data_ptr(), None if entropy is None else entropy.data_ptr(), None if place is None else place.data_ptr(), k,
+              ids, best, top_pitch, _stream_here(here))
+    _check(lib, code, "token_logprobs")
 
 
 # ---------------------------------------------------------------------------

@@ -11,25 +11,24 @@ def host(monkeypatch):
     class Launched(Exception):
         pass
 
-    class Library:
-        def __getattr__(self, name):
-            if name == "sglc_attention_prefix_workspace":
-                class Size:
-                    restype = None
+    def function(library, name, types, result=None):
+        def sizes(T, G, H, Hkv, D, dt):
+            assert len(types) == 6
+            return 1000 if H % Hkv == 0 and D % 8 == 0 and D <= 256 and G <= ops.PREFIX_GROUPS else -1
 
-                    def __call__(self, T, G, H, Hkv, D, dt):
-                        return 1000 if H % Hkv == 0 and D % 8 == 0 and D <= 256 and G <= ops.PREFIX_GROUPS else -1
-                return Size()
+        def launch(*args):
+            assert len(args) == len(types)
+            for a, t in zip(args, types):
+                assert isinstance(a, float if t == "f" else (int, type(None)) if t == "p" else int), (name, t, a)
+            raise Launched
+        return None, sizes if name == "sglc_attention_prefix_workspace" else launch
 
-            def launch(*args):
-                raise Launched
-            return launch
-
-    monkeypatch.setattr(ops, "_need_cuda", lambda *t: None)
-    monkeypatch.setattr(ops, "_on_current_device", lambda what, *t: None)
-    monkeypatch.setattr(ops, "_stream", lambda: None)
-    monkeypatch.setattr(ops, "tc_error_flag", lambda device: None)
-    monkeypatch.setattr(build, "load", lambda name: Library())
+    monkeypatch.setattr(ops, "_here", lambda what, *t: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(ops, "_prefix_sizes", {})
+    monkeypatch.setattr(ops, "_stream_here", lambda device: 0)
+    monkeypatch.setattr(ops, "tc_error_flag", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(ops, "_function", function)
     return Launched
 
 
@@ -122,7 +121,8 @@ def _logprobs(**kw):
     (dict(top_ids=_i32(4, 65), top_logprobs=torch.zeros(4, 65)), "at most 64"),
     (dict(logits=torch.zeros(4, 2)), "3 alternatives of 2"),
     (dict(top_ids=_i32(4, 6)[:, ::2], top_logprobs=torch.zeros(4, 6)[:, ::2]), "one stride"),
-    (dict(top_ids=_i32(4, 5)[:, :3]), "one stride")])
+    (dict(top_ids=_i32(4, 5)[:, :3]), "one stride"),
+    (dict(top_ids=_i32(1, 3).expand(4, 3), top_logprobs=torch.zeros(1, 3).expand(4, 3)), "overlap")])
 def test_token_logprobs_refuses(host, kw, words):
     with pytest.raises(host):
         _logprobs()
@@ -132,7 +132,8 @@ def test_token_logprobs_refuses(host, kw, words):
         _logprobs(**kw)
 
 
-def test_they_refuse_tensors_of_the_host():
+def test_they_refuse_tensors_of_the_host(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     for call in (_tables, _prefix, _logprobs):
         with pytest.raises(ops.KernelError, match="CUDA tensors only"):
             call()
