@@ -20,14 +20,17 @@ namespace {
 using namespace prefix;
 
 // ---- prefixes, 32-bit arithmetic (any head size that is a multiple of 8, up to 256) -----------------------------------------
-// A tile of 64 rows by 64 keys: a thread has 4 x 4 scores, fed by 16-byte reads of queries and keys from shared memory (8 for
-// 64 multiply-adds), and 4 rows by D / 16 columns of the sums.
+// A tile of 16 R rows by 64 keys: a thread has R x 4 scores, fed by 16-byte reads of queries and keys from shared memory (for R
+// = 4 eight for 64 multiply-adds), and R rows by D / 16 columns of the sums.  R = 4 where groups have many rows; R = 1 where
+// they have up to 32: most of 64 rows would be empty, and what bounds such a call is the time of a few tiles (22 requests of
+// 12 heads on two prefixes of 1,000: GENERAL_TIME).
 constexpr int GT = 256;                   // threads
-constexpr int GR = GENERAL_ROWS, GK = GENERAL_KEYS;
+constexpr int GK = GENERAL_KEYS;
 
-template <typename T, int NC>             // NC: blocks of 64 columns
+template <typename T, int NC, int R>      // NC: blocks of 64 columns
 __global__ void __launch_bounds__(GT)
 prefix_general_kernel(const Args a) {
+  constexpr int GR = 16 * R;
   extern __shared__ __align__(16) float sm[];
   const int D = a.D, DS = D + 4;          // (rows of queries and keys four words apart from the banks' period)
   float* sQ = sm;                         // [GR][DS]
@@ -35,7 +38,7 @@ prefix_general_kernel(const Args a) {
   float* sV = sK + GK * DS;               // [GK][NC * 64]
   float* sP = sV + GK * NC * 64;          // [GR][GK + 4]
   __shared__ Plan plan;
-  __shared__ int lim[GR];
+  __shared__ int lim[GR], sPage[GK];
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   pdl_wait();
   pdl_launch_dependents();                // (here and not before: the second launch reads what came before this one)
@@ -59,9 +62,9 @@ prefix_general_kernel(const Args a) {
       for (int i = 0; i < 8; i++) sQ[row * DS + d + i] = v[i];
     }
     if (tid < GR) lim[tid] = tid < rows ? visible(a, s.t0 + (row0 + tid) / gq, s.keys) : 0;
-    float m[4], l[4], o[4][NC][4];
+    float m[R], l[R], o[R][NC][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < R; i++) {
       m[i] = -INFINITY;
       l[i] = 0.0f;
 #pragma unroll
@@ -69,42 +72,56 @@ prefix_general_kernel(const Args a) {
 #pragma unroll
         for (int u = 0; u < 4; u++) o[i][c][u] = 0.0f;
     }
+    // (a tile's pages are looked up a tile ahead)
+    auto page_id = [&](int j) {
+      const int key = (s.tile + j) * GK + tid;
+      return tid < GK && j < s.tiles && key < s.keys ? page_of(a, req, key) : -1;
+    };
+    int page_next = page_id(0);
     for (int j = 0; j < s.tiles; j++) {
       const int key0 = (s.tile + j) * GK;
       __syncthreads();
-      for (int x = tid; x < GK * NC * 8; x += GT) {
-        const int row = x / (NC * 8), d = x % (NC * 8) * 8, key = key0 + row;
-        float k[8], v[8];
+      if (tid < GK) sPage[tid] = page_next;
+      __syncthreads();
+      page_next = page_id(j + 1);
 #pragma unroll
-        for (int i = 0; i < 8; i++) k[i] = v[i] = 0.0f;
-        if (d < D && key < s.keys) {
-          const int page = page_of(a, req, key);
-          if (page >= 0) {
-            const size_t at = row_at(a, page, s.hk, key) + d;
-            load8(reinterpret_cast<const T*>(a.cache) + at, 1, k);
-            load8(reinterpret_cast<const T*>(a.cache) + at + value_offset(a), 1, v);
+      for (int x0 = 0; x0 < GK * NC * 8; x0 += 2 * GT) {       // (two pieces of keys and of values on their way a thread)
+        float k[2][8], v[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int x = x0 + u * GT + tid, row = x / (NC * 8), d = x % (NC * 8) * 8, page = sPage[row];
+#pragma unroll
+          for (int i = 0; i < 8; i++) k[u][i] = v[u][i] = 0.0f;
+          if (d < D && page >= 0) {
+            const size_t at = row_at(a, page, s.hk, key0 + row) + d;
+            load8(reinterpret_cast<const T*>(a.cache) + at, 1, k[u]);
+            load8(reinterpret_cast<const T*>(a.cache) + at + value_offset(a), 1, v[u]);
           }
         }
-        if (d < D)
 #pragma unroll
-          for (int i = 0; i < 8; i++) sK[row * DS + d + i] = k[i];
+        for (int u = 0; u < 2; u++) {
+          const int x = x0 + u * GT + tid, row = x / (NC * 8), d = x % (NC * 8) * 8;
+          if (d < D)
 #pragma unroll
-        for (int i = 0; i < 8; i++) sV[row * NC * 64 + d + i] = v[i];
+            for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(&sK[row * DS + d + i]) = make_float4(k[u][i], k[u][i + 1], k[u][i + 2], k[u][i + 3]);
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(&sV[row * NC * 64 + d + i]) = make_float4(v[u][i], v[u][i + 1], v[u][i + 2], v[u][i + 3]);
+        }
       }
       __syncthreads();
-      float x[4][4];
+      float x[R][4];
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int i = 0; i < R; i++)
 #pragma unroll
         for (int u = 0; u < 4; u++) x[i][u] = 0.0f;
       for (int d = 0; d < D; d += 4) {
-        float4 q4[4], k4[4];
+        float4 q4[R], k4[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) q4[i] = *reinterpret_cast<const float4*>(&sQ[(ty * 4 + i) * DS + d]);
+        for (int i = 0; i < R; i++) q4[i] = *reinterpret_cast<const float4*>(&sQ[(ty * R + i) * DS + d]);
 #pragma unroll
         for (int u = 0; u < 4; u++) k4[u] = *reinterpret_cast<const float4*>(&sK[(tx + 16 * u) * DS + d]);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < R; i++)
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             x[i][u] = fmaf(q4[i].x, k4[u].x, x[i][u]);
@@ -114,8 +131,8 @@ prefix_general_kernel(const Args a) {
           }
       }
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int row = ty * 4 + i, n = lim[row] - key0;      // keys of this tile that the row sees
+      for (int i = 0; i < R; i++) {
+        const int row = ty * R + i, n = lim[row] - key0;      // keys of this tile that the row sees
         float mx = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -145,16 +162,16 @@ prefix_general_kernel(const Args a) {
       __syncwarp();                       // (a row's weights are made and used by the same half of a warp)
 #pragma unroll 2
       for (int key = 0; key < GK; key += 4) {
-        float4 p4[4];
+        float4 p4[R];
 #pragma unroll
-        for (int i = 0; i < 4; i++) p4[i] = *reinterpret_cast<const float4*>(&sP[(ty * 4 + i) * (GK + 4) + key]);
+        for (int i = 0; i < R; i++) p4[i] = *reinterpret_cast<const float4*>(&sP[(ty * R + i) * (GK + 4) + key]);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
           float4 v4[4];
 #pragma unroll
           for (int u = 0; u < 4; u++) v4[u] = *reinterpret_cast<const float4*>(&sV[(key + u) * NC * 64 + c * 64 + tx * 4]);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
+          for (int i = 0; i < R; i++) {
             const float w[4] = {p4[i].x, p4[i].y, p4[i].z, p4[i].w};
 #pragma unroll
             for (int u = 0; u < 4; u++) {
@@ -170,8 +187,8 @@ prefix_general_kernel(const Args a) {
     if (tid == 0) record_item(a, s);
     const size_t slot = (size_t)(blockIdx.x + s.item) * a.slot_rows;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int row = ty * 4 + i;
+    for (int i = 0; i < R; i++) {
+      const int row = ty * R + i;
 #pragma unroll
       for (int w = 1; w < 16; w <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
       if (row < rows && slot_ok(a, s)) {
@@ -245,7 +262,7 @@ __host__ __device__ constexpr int round_keys(int size, int HC, int LW) {
 
 // LW: lanes of a row.  WARPS: of an item; a block has four.
 template <typename T, int HC, int LW, int WARPS>
-__global__ void __launch_bounds__(OT)
+__global__ void __launch_bounds__(OT, HC == 1 ? 6 : HC == 2 ? 4 : 3)
 prefix_own_kernel(const Args a) {
   extern __shared__ __align__(16) float sm[];          // [4 warps][HC][D + 2], then [HC][warps of an item]: for items of several
   constexpr int per_warp = 32 / LW, ITEMS = 4 / WARPS;
@@ -487,21 +504,26 @@ prefix_own_kernel(const Args a) {
   }
 }
 
-template <typename T, int NC>
+template <typename T, int NC, int R>
 int launch_general(const Args& a, cudaStream_t stream) {
+  constexpr int GR = 16 * R;
   const size_t smem = (size_t)((GR + GK) * (a.D + 4) + GK * NC * 64 + GR * (GK + 4)) * 4;
-  const cudaError_t e = cudaFuncSetAttribute(prefix_general_kernel<T, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  const cudaError_t e = cudaFuncSetAttribute(prefix_general_kernel<T, NC, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              ((GR + GK) * (NC * 64 + 4) + GK * NC * 64 + GR * (GK + 4)) * 4);
   if (e != cudaSuccess) return (int)e;
-  return sglc_launch(prefix_general_kernel<T, NC>, dim3(a.n_blocks), dim3(GT), smem, stream, 1, true, a);
+  return sglc_launch(prefix_general_kernel<T, NC, R>, dim3(a.n_blocks), dim3(GT), smem, stream, 1, true, a);
+}
+template <typename T, int NC>
+int rows_general(const Args& a, cudaStream_t stream) {
+  return a.row_shift == 4 ? launch_general<T, NC, 1>(a, stream) : launch_general<T, NC, 4>(a, stream);
 }
 template <typename T>
 int run_general(const Args& a, cudaStream_t stream) {
   switch ((a.D + 63) / 64) {
-    case 1: return launch_general<T, 1>(a, stream);
-    case 2: return launch_general<T, 2>(a, stream);
-    case 3: return launch_general<T, 3>(a, stream);
-    default: return launch_general<T, 4>(a, stream);
+    case 1: return rows_general<T, 1>(a, stream);
+    case 2: return rows_general<T, 2>(a, stream);
+    case 3: return rows_general<T, 3>(a, stream);
+    default: return rows_general<T, 4>(a, stream);
   }
 }
 
@@ -553,12 +575,13 @@ int multiprocessors() {
 bool lay_out(Args* a, int dtype) {
   a->sms = multiprocessors();
   if (a->sms <= 0) return false;
+  a->gq = a->H / a->Hkv;
   a->tc = dtype == SGLC_BF16 && (a->D == 64 || a->D == 128);
   a->n_blocks = a->tc ? a->sms : 2 * a->sms;
-  a->slot_rows = a->tc ? TC_SLOT : GENERAL_ROWS;
-  a->gq = a->H / a->Hkv;
+  a->row_shift = (long long)a->T * a->gq <= 32LL * a->G ? 4 : 6;             // (rows of a group's key head, on average)
+  a->slot_rows = a->tc ? TC_SLOT : 1 << a->row_shift;
   a->key_shift = a->tc ? 7 : 6;
-  static_assert(TC_KEYS == 128 && GENERAL_KEYS == 64 && GENERAL_ROWS == 64, "as the shifts say");
+  static_assert(TC_KEYS == 128 && GENERAL_KEYS == 64, "as the shift says");
   const long long rows = (long long)a->T * a->gq;
   a->slots = a->n_blocks + a->Hkv * (rows / a->slot_rows + a->G);      // (items of 128 rows are the only ones of their group)
   a->lanes = 1;

@@ -5,7 +5,7 @@
 
 namespace prefix {
 constexpr int MAX_GROUPS = 256;
-constexpr int GENERAL_ROWS = 64, GENERAL_KEYS = 64;       // an item's rows, a tile's keys
+constexpr int GENERAL_KEYS = 64;          // a tile's keys in 32-bit arithmetic
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -25,7 +25,7 @@ struct Args {
   float scale;
   int* err;
   // the launch
-  int sms, n_blocks, slot_rows, key_shift, lanes;        // key_shift: log2 of a tile's keys
+  int sms, n_blocks, slot_rows, key_shift, row_shift, lanes;       // log2 of a tile's keys, of an item's rows (not tc)
   int tc;                                 // the tensor-core kernel
   long long slots;
   float* part_o;                          // [slots][slot_rows][D]: sums, against a maximum
@@ -75,7 +75,7 @@ __device__ __forceinline__ void group_tokens(const Args& a, int g, int& t0, int&
 __device__ __forceinline__ int prefix_length(const Args& a, int g) { return min(max(a.shared_len[g], 0), a.last_position + 1); }
 
 // Rows of an item of a group of so many rows a key head, as a power of two.
-__device__ __forceinline__ int item_shift(const Args& a, int rows) { return !a.tc ? 6 : rows <= 128 ? 7 : 8; }
+__device__ __forceinline__ int item_shift(const Args& a, int rows) { return !a.tc ? a.row_shift : rows <= 128 ? 7 : 8; }
 __device__ __forceinline__ int items_of(const Args& a, int rows) { return (int)(((long long)rows + (1 << item_shift(a, rows)) - 1) >> item_shift(a, rows)); }
 __device__ __forceinline__ int tiles_of_keys(const Args& a, int keys) { return (keys + (1 << a.key_shift) - 1) >> a.key_shift; }
 // (a division of 64 bits takes a hundred instructions)
