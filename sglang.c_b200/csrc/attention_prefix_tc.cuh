@@ -109,25 +109,26 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
   const int gq = a.gq;
 
   if (warp >= TC_LOAD_WARP) {
-    // ---- loads, a warp for keys and one for values: a lane a box, whose page is asked for a tile ahead ----
+    // ---- loads, a warp for keys and one for values: a lane a box ----
     // (a copy takes a warp's turn for 200 cycles, whoever issues it: 16 pages of 16 rows a tile were 3,250 cycles in one warp)
     const int half = warp - TC_LOAD_WARP;
     uint8_t* mine = ring + half * RING * UNIT;
+    // A lane holds the page of one of 32 boxes, and of one of the 32 behind them: a look into the table takes longer than a
+    // tile's copies, and with one a tile ahead the loads were what the others waited for.
     Segment s = first_segment(a, plan);
-    int j = 0;
-    int req = keeper(a, s);
-    auto page_id = [&](const Segment& x, int jj, int b) {
-      const int key = (x.tile + jj) * TC_KEYS + b * box;
-      if (x.tiles <= 0 || b * box >= TC_KEYS || key >= x.keys) return -1;
-      const int page = page_of(a, req, key);
+    int j = 0, req = keeper(a, s);
+    auto page_id = [&](int b) {                     // box b from the piece's first key on
+      const long long key = (long long)s.tile * TC_KEYS + (long long)b * box;
+      if (key >= s.keys || key >= (long long)(s.tile + s.tiles) * TC_KEYS) return -1;
+      const int page = page_of(a, req, (int)key);
       return page < 0 ? a.n_pages : page;           // (a page outside reads as zeros)
     };
-    int id_next = page_id(s, 0, lane);
+    const int of_tile = TC_KEYS / box;
+    int id = page_id(lane), id_next = page_id(32 + lane), held = 0;
     uint32_t u = 0;
     bool ok = true;
     for (; s.tiles > 0; u++) {
-      const int id = id_next, slot = u % RING;
-      const int key0 = (s.tile + j) * TC_KEYS, boxes = (min(TC_KEYS, s.keys - key0) + box - 1) / box;
+      const int slot = u % RING, key0 = (s.tile + j) * TC_KEYS, boxes = (min(TC_KEYS, s.keys - key0) + box - 1) / box;
       if (u >= RING) {
         int w = 1;
         if (lane == 0) w = mbar_wait(&ctl.empty[half][slot], (u / RING - 1) & 1, abort_flag) ? 1 : 0;
@@ -136,18 +137,31 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       }
       if (lane == 0) mbar_expect_tx(&ctl.full[half][slot], (uint32_t)boxes * DB * box * 128u);
       __syncwarp();
-      for (int b = lane; b < boxes; b += 32) {
-        const int page = b < 32 ? id : page_id(s, j, b), in_page = (key0 + b * box) % a.page_size;
-        for (int blk = 0; blk < DB; blk++)
-          tma_load_5d(mine + slot * UNIT + blk * TC_TILE + b * box * 128, &map_kv, &ctl.full[half][slot], blk * 64, in_page, s.hk, half,
-                      page);
+      for (int b0 = 0; b0 < boxes; b0 += 32) {
+        const int first = j * of_tile + b0;         // (a multiple of the tile's boxes, or of 32)
+        if (first >= held + 32) {
+          held += 32;
+          id = id_next;
+          id_next = page_id(held + 32 + lane);
+        }
+        const int page = __shfl_sync(0xffffffffu, id, (first - held + lane) & 31), b = b0 + lane;
+        if (b < boxes && lane < of_tile) {
+          const int in_page = (key0 + b * box) % a.page_size;
+#pragma unroll
+          for (int blk = 0; blk < DB; blk++)
+            tma_load_5d(mine + slot * UNIT + blk * TC_TILE + b * box * 128, &map_kv, &ctl.full[half][slot], blk * 64, in_page, s.hk, half,
+                        page);
+        }
       }
       if (++j == s.tiles) {
         s = next_segment(a, plan, s);
         req = keeper(a, s);
-        j = 0;
+        j = held = 0;
+        if (s.tiles > 0) {
+          id = page_id(lane);
+          id_next = page_id(32 + lane);
+        }
       }
-      id_next = page_id(s, j, lane);
     }
     if (!ok)                                        // given up: what is still on its way here lands first (a limit again)
       for (uint32_t z = u - RING; z < u; z++)
@@ -168,14 +182,14 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       bool ok = true;
       for (Segment s = first_segment(a, plan); s.tiles > 0 && ok; s = next_segment(a, plan, s)) {
         const bool pair = s.shift == 8;
-        const uint32_t q_at = smem_u32(sQ) + (pair ? w * UNIT : 0);
+        const uint32_t q_at = smem_u32(sQ) + w * UNIT;
         ok = mbar_wait(&ctl.q_full, q_turn & 1, abort_flag);
         if (!ok) break;
         q_turn++;
         // a tile is given back when both groups have taken it: where it is this one's alone, by two arrivals
         auto give_back = [&](uint64_t* bar) {
           mma_commit(bar);
-          if (!pair) mma_commit(bar);
+          if (!pair) mbar_arrive(bar);
         };
         auto scores = [&](int i) {
           const uint32_t u = u0 + tile_of(pair, w, i >> 1), slot = u % RING;
@@ -225,7 +239,9 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
     for (Segment s = first_segment(a, plan); s.tiles > 0; s = next_segment(a, plan, s)) {
       const bool pair = s.shift == 8;
       const int rows = min(1 << s.shift, s.n_rows - s.row0);         // of this item
-      const int mine = pair ? w * TC_WG + row : row;
+      // (where both groups have the same rows, the second has them 64 lanes on: up to 64 rows then keep all four schedulers
+      // busy, not two of them twice)
+      const int mine = pair ? w * TC_WG + row : (row + w * 64) & (TC_WG - 1);
       const int n = s.row0 + mine, t = s.t0 + (unsigned)n / (unsigned)gq;
       const bool valid = mine < rows;
       const int lim = valid ? visible(a, t, s.keys) : 0;
@@ -254,12 +270,16 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
 #pragma unroll
         for (int u = 0; u < 8; u++) {
           const int at = x0 + u * 2 * TC_WG, r = at / (D / 8), c = at % (D / 8);
-          if (r < 1 << s.shift) *reinterpret_cast<uint4*>(sQ + (r / TC_WG) * UNIT + (c / 8) * TC_TILE + sw128(r % TC_WG, c % 8)) = x[u];
+          if (r < 1 << s.shift) {
+            uint8_t* to = sQ + (c / 8) * TC_TILE;
+            *reinterpret_cast<uint4*>(to + (r / TC_WG) * UNIT + sw128(r % TC_WG, c % 8)) = x[u];
+            if (!pair) *reinterpret_cast<uint4*>(to + UNIT + sw128((r + 64) & (TC_WG - 1), c % 8)) = x[u];
+          }
         }
       }
       fence_async_proxy();
       mbar_arrive(&ctl.q_full);
-      const bool busy = (warp & 3) * 32 + (pair ? w * TC_WG : 0) < rows;       // this warp has rows at all
+      const bool busy = (mine & ~31) < rows;         // this warp has rows at all
       const int steps = 2 * tiles_of(pair, s.tiles, w);
       float m = -INFINITY, l = 0.0f;
       for (int i = 0; i < steps && ok; i++, turn++) {
