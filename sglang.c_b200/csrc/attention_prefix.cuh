@@ -1,6 +1,8 @@
 // What the launches of attention over shared prefixes agree on: the plan of items and shares that each block makes from
 // the groups' lengths, where parts lie in the workspace, and access to the paged cache with every index checked.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace prefix {
@@ -277,5 +279,19 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, int vec, const float (&
 #pragma unroll
     for (int i = 0; i < 8; i++) p[i] = __float2bfloat16_rn(v[i]);
   }
+}
+
+// Lets a kernel take so much shared memory, once a device (a bit each; beyond 64 of them at every call).
+template <typename... KArgs>
+static int allow_shared(void (*kernel)(KArgs...), int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return (int)e;
+  done.fetch_or(bit, std::memory_order_release);
+  return 0;
 }
 }  // namespace prefix

@@ -230,28 +230,40 @@ prefix_join_kernel(const Args a, int tokens, int heads) {
   const int s0 = __shfl_sync(0xffffffffu, t0, row_token[0] & 31), s1 = __shfl_sync(0xffffffffu, t0, row_token[1] & 31);
   const int e0 = __shfl_sync(0xffffffffu, t1, row_token[0] & 31), e1 = __shfl_sync(0xffffffffu, t1, row_token[1] & 31);
   pdl_wait();                                          // the prefixes' parts are there
+  // (both rows' parts together: a part is a chain of three reads)
+  Parts ps[2];
 #pragma unroll
   for (int x = 0; x < 2; x++) {
+    ps[x].n = 0;
     if (!row_in[x] || row_lo[x] == 0) continue;
     const int from = x ? s1 : s0, h = g + 8 * x - row_token[x] * heads;
-    const Parts ps = parts_of(a, x ? g1 : g0, from, x ? e1 : e0, hk, (t_first + row_token[x] - from) * a.gq + head0 + h);
-    for (int j = walker; j < ps.n; j += walkers) {
-      const long long at = part_row(a, ps, j);
-      if (at < 0) continue;
-      const float2 ml = a.part_ml[at];
-      float4 v[B][2];
+    ps[x] = parts_of(a, x ? g1 : g0, from, x ? e1 : e0, hk, (t_first + row_token[x] - from) * a.gq + head0 + h);
+  }
+  for (int j = walker; j < max(ps[0].n, ps[1].n); j += walkers) {
+    float2 ml[2];
+    float4 v[2][B][2];
 #pragma unroll
-      for (int b = 0; b < B; b++) {
-        v[b][0] = *reinterpret_cast<const float4*>(a.part_o + at * D + 32 * b + 8 * q);
-        v[b][1] = *reinterpret_cast<const float4*>(a.part_o + at * D + 32 * b + 8 * q + 4);
+    for (int x = 0; x < 2; x++) {
+      const long long at = j < ps[x].n ? part_row(a, ps[x], j) : -1;
+      ml[x] = make_float2(-INFINITY, 0.0f);
+      if (at >= 0) {
+        ml[x] = a.part_ml[at];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+          v[x][b][0] = *reinterpret_cast<const float4*>(a.part_o + at * D + 32 * b + 8 * q);
+          v[x][b][1] = *reinterpret_cast<const float4*>(a.part_o + at * D + 32 * b + 8 * q + 4);
+        }
       }
-      if (ml.y == 0.0f) continue;                      // nothing was seen and no sums were written (NaN is not 0)
-      const float top = fmaxf(m[x], ml.x), ref = top == -INFINITY ? 0.0f : top, f = ex2(m[x] - ref), f2 = ex2(ml.x - ref);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      if (ml[x].y == 0.0f) continue;                   // nothing was seen and no sums were written (NaN is not 0)
+      const float top = fmaxf(m[x], ml[x].x), ref = top == -INFINITY ? 0.0f : top, f = ex2(m[x] - ref), f2 = ex2(ml[x].x - ref);
       m[x] = top;
-      l[x] = l[x] * f + ml.y * f2;
+      l[x] = l[x] * f + ml[x].y * f2;
 #pragma unroll
       for (int b = 0; b < B; b++) {
-        const float w[8] = {v[b][0].x, v[b][0].y, v[b][0].z, v[b][0].w, v[b][1].x, v[b][1].y, v[b][1].z, v[b][1].w};
+        const float w[8] = {v[x][b][0].x, v[x][b][0].y, v[x][b][0].z, v[x][b][0].w, v[x][b][1].x, v[x][b][1].y, v[x][b][1].z, v[x][b][1].w};
 #pragma unroll
         for (int i = 0; i < 8; i++) o[b][i >> 1][2 * x + (i & 1)] = o[b][i >> 1][2 * x + (i & 1)] * f + w[i] * f2;
       }

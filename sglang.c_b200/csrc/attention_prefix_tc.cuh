@@ -420,8 +420,9 @@ int launch_tc(const Args& a, cudaStream_t stream) {
   CUtensorMap map;
   memset(&map, 0, sizeof(map));
   if (!make_kv_map(&map, a, box)) return SGLC_ERR_UNSUPPORTED;
-  const cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<D, RING>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  static std::atomic<unsigned long long> done{0};
+  const int code = allow_shared(prefix_tc_kernel<D, RING>, (int)smem, done);
+  if (code) return code;
   return sglc_launch(prefix_tc_kernel<D, RING>, dim3(a.n_blocks), dim3(TC_THREADS), smem, stream, 1, true, map, a, box);
 }
 }  // namespace prefix

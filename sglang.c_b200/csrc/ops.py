@@ -317,6 +317,7 @@ def kv_write(k_src, v_src, cache, slots, n_kv_heads, head_dim):
 
 
 _INT, _FLOAT = torch.int32, torch.float32
+_MOST = 1 << 29              # rows, tokens or entries of a row that the launchers below take (they count in 32 bits)
 _functions = {}              # (library, launcher) -> the ctypes function with its argument types declared
 
 
@@ -373,8 +374,8 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
             names = ("q_len", "kv_len", "free_pages", "n_free", "q_start", "new_len", "token_req", "positions", "slots", "left", "status")
             _i32(t, f"step_tables: {next(n for n, x in zip(names, arrays) if x is t)}")
     R, T = q_len.numel(), token_req.numel()
-    if R > STEP_TABLES_REQUESTS:
-        raise KernelError(f"step_tables: {R} requests; at most {STEP_TABLES_REQUESTS}")
+    if R > STEP_TABLES_REQUESTS or T > _MOST or free_pages.numel() > _MOST:
+        raise KernelError(f"step_tables: {R} requests, {T} tokens; at most {STEP_TABLES_REQUESTS} and {_MOST}")
     if block_table.dtype is not _INT or block_table.dim() != 2:
         raise KernelError(f"step_tables: block_table must be int32 rows for {R} requests")
     (rows, width), (pitch, column) = block_table.shape, block_table.stride()
@@ -836,6 +837,8 @@ def attention_prefix(q, cache, block_table, token_req, positions, group_start, s
     if q.dim() != 2 or out.dim() != 2:
         raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
     (T, q_width), (q_pitch, q_column), (rows, width), (pitch, column) = q.shape, q.stride(), out.shape, out.stride()
+    if T > _MOST or cache.numel() == 0:
+        raise KernelError(f"attention_prefix: {T} tokens (at most {_MOST}), a cache of {n_pages} pages of {page_size}")
     if q_width != n_heads * D or width != q_width or rows < T or q_column != 1 or column != 1:
         raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
     if rows > 1 and pitch < width:
@@ -955,6 +958,8 @@ def token_logprobs(logits, tokens, logprob, entropy=None, place=None, top_ids=No
     (n, V), (pitch, column) = logits.shape, logits.stride()
     if V < 1 or (V > 1 and column != 1):
         raise KernelError("token_logprobs: logits must be rows of a vocabulary")
+    if n > _MOST or V > _MOST:
+        raise KernelError(f"token_logprobs: {n} rows of {V}; at most {_MOST} both")
     for t, dt, nm in ((tokens, _INT, "tokens"), (logprob, _FLOAT, "logprob"), (entropy, _FLOAT, "entropy"), (place, _INT, "place")):
         if t is None and nm != "logprob":
             continue

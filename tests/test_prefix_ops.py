@@ -139,6 +139,33 @@ def test_they_refuse_tensors_of_the_host(monkeypatch):
             call()
 
 
+def test_they_refuse_tensors_of_another_device(monkeypatch):
+    """Tensors of device 1 while device 0 is current: the kernels would run on the wrong one's stream."""
+    class There:
+        device, is_cuda = "cuda:1", True
+
+        def get_device(self):
+            return 1
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    assert ops._here("x", None) == 0
+    with pytest.raises(ops.KernelError, match="lies on cuda:1, the current device is cuda:0"):
+        ops._here("x", None, There())
+
+
+def test_sizes_beyond_32_bits_are_refused(host):
+    """(Tensors of torch's device without memory.)"""
+    for shape in ((4, 1 << 30), (1 << 30, 1)):
+        logits = torch.empty(shape, device="meta")
+        with pytest.raises(ops.KernelError, match="at most 536870912 both"):
+            _logprobs(logits=logits)
+    with pytest.raises(ops.KernelError, match="at most 536870912"):
+        _prefix(q=torch.empty((1 << 30, 48), device="meta"))
+    with pytest.raises(ops.KernelError, match="at most 16384 and 536870912"):
+        _tables(token_req=torch.empty(1 << 30, dtype=torch.int32, device="meta"))
+    with pytest.raises(ops.KernelError, match="a cache of 0 pages"):
+        _prefix(cache=torch.zeros(0, 2, 2, 4, 8))
+
+
 def test_the_sizes_named_here_are_the_kernels():
     """What the bindings say of limits is what the sources say."""
     import os
