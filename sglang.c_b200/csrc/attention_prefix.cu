@@ -19,7 +19,7 @@ SGLC_DEFINE_ERROR_STRING()
 namespace {
 using namespace prefix;
 
-// ---- prefixes, 32-bit arithmetic (any head size that is a multiple of 8, up to 256) -----------------------------------------
+// ---- prefixes, 32-bit arithmetic: float32, and bfloat16 heads of more than 128 ------------------------------------------------
 // A tile of 16 R rows by 64 keys: a thread has R x 4 scores, fed by 16-byte reads of queries and keys from shared memory (for R
 // = 4 eight for 64 multiply-adds), and R rows by D / 16 columns of the sums.  R = 4 where groups have many rows; R = 1 where
 // they have up to 32: most of 64 rows would be empty, and what bounds such a call is the time of a few tiles (22 requests of
@@ -519,12 +519,11 @@ int rows_general(const Args& a, cudaStream_t stream) {
 }
 template <typename T>
 int run_general(const Args& a, cudaStream_t stream) {
-  switch ((a.D + 63) / 64) {
-    case 1: return rows_general<T, 1>(a, stream);
-    case 2: return rows_general<T, 2>(a, stream);
-    case 3: return rows_general<T, 3>(a, stream);
-    default: return rows_general<T, 4>(a, stream);
+  if constexpr (sizeof(T) == 4) {                      // (bfloat16 heads of up to 128: the tensor cores')
+    if (a.D <= 64) return rows_general<T, 1>(a, stream);
+    if (a.D <= 128) return rows_general<T, 2>(a, stream);
   }
+  return a.D <= 192 ? rows_general<T, 3>(a, stream) : rows_general<T, 4>(a, stream);
 }
 
 template <typename T, int HC, int LW, int WARPS>
@@ -576,7 +575,7 @@ bool lay_out(Args* a, int dtype) {
   a->sms = multiprocessors();
   if (a->sms <= 0) return false;
   a->gq = a->H / a->Hkv;
-  a->tc = dtype == SGLC_BF16 && (a->D == 64 || a->D == 128);
+  a->tc = dtype == SGLC_BF16 && a->D <= 128;
   a->n_blocks = a->tc ? a->sms : 2 * a->sms;
   a->row_shift = (long long)a->T * a->gq <= 32LL * a->G ? 4 : 6;             // (rows of a group's key head, on average)
   a->slot_rows = a->tc ? TC_SLOT : 1 << a->row_shift;
@@ -639,7 +638,7 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   a.first_item = reinterpret_cast<int*>(a.part_ml + a.slots * a.slot_rows);
   a.item_blocks = reinterpret_cast<int2*>(a.first_item + (G + 1) / 2 * 2);
   a.o_vec = ((uintptr_t)out & 15) == 0 && o_stride * (dtype == SGLC_F32 ? 4 : 2) % 16 == 0;
-  const int code = a.tc ? (D == 64 ? launch_tc<64, 4>(a, stream) : launch_tc<128, 2>(a, stream))
+  const int code = a.tc ? (D <= 64 ? launch_tc<64, 4>(a, stream) : launch_tc<128, 2>(a, stream))
                         : dtype == SGLC_F32 ? run_general<float>(a, stream) : run_general<__nv_bfloat16>(a, stream);
   if (code) return code;
   if (join_pays(a)) return D == 64 ? run_join<64>(a, max_own, stream) : run_join<128>(a, max_own, stream);

@@ -203,14 +203,13 @@ prefix_join_kernel(const Args a, int tokens, int heads) {
       uint32_t p[4];
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-        float e[4];
+        // (sums of the rounded weights, which the values get)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          e[i] = ex2(s[x][i] - ref[i >> 1]);
-          l[i >> 1] += e[i];
+        for (int y = 0; y < 2; y++) {
+          const uint32_t w = pack_bf16(ex2(s[x][2 * y] - ref[y]), ex2(s[x][2 * y + 1] - ref[y]));
+          l[y] += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
+          p[2 * x + y] = w;
         }
-        p[2 * x] = pack_bf16(e[0], e[1]);
-        p[2 * x + 1] = pack_bf16(e[2], e[3]);
       }
 #pragma unroll
       for (int b = 0; b < B; b++) {
@@ -373,7 +372,7 @@ static inline int join_tokens(const Args& a) {
 // Four rows an item and more: below, the 16 rows of the instruction are mostly empty and the multiply-add kernel wins (64
 // requests of 25 heads of one: 55 against 44 us for the whole call, 100 of 16 heads over 8: 36 against 27; 256 of
 // 32 heads over 8: 187 against 205).
-static inline bool join_pays(const Args& a) { return a.tc && join_tokens(a) * a.gq >= 4; }
+static inline bool join_pays(const Args& a) { return a.tc && (a.D == 64 || a.D == 128) && join_tokens(a) * a.gq >= 4; }
 // Warps an item: one where the items fill the multiprocessors' warps, else two, else four, and blocks of a
 // cluster while there are fewer than four a multiprocessor and 64 keys or more are left for each.
 template <int D>

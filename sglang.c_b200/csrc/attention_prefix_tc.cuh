@@ -1,4 +1,5 @@
-// The prefixes' parts of attention over shared prefixes on the tensor cores: bfloat16, head sizes 64 and 128.
+// The prefixes' parts of attention over shared prefixes on the tensor cores: bfloat16, head sizes up to 128 (multiples of 8; in
+// tiles of 64 or 128 columns, zeros behind a head's own: its last columns lie outside of the tensor that the copies read).
 //
 // One block per multiprocessor, a share of the tiles of 128 keys each (see the plan).  Scores S = Q K^T of 128 rows by 128 keys
 // go into tensor memory; a thread has a row of them, takes its maximum, turns them into bfloat16 weights
@@ -255,9 +256,9 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
         for (int u = 0; u < 8; u++) {
           const int at = x0 + u * 2 * TC_WG, r = at / (D / 8), c = at % (D / 8);
           x[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows) {
+          if (r < rows && c * 8 < a.D) {
             const int nr = s.row0 + r, tr = (unsigned)nr / (unsigned)gq;
-            const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(s.t0 + tr) * a.q_stride + (size_t)(s.hk * gq + nr - tr * gq) * D + c * 8;
+            const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(s.t0 + tr) * a.q_stride + (size_t)(s.hk * gq + nr - tr * gq) * a.D + c * 8;
             if (a.q_vec) {
               x[u] = *reinterpret_cast<const uint4*>(from);
             } else {
@@ -332,10 +333,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
           for (int x = 0; x < 32; x++) {
             const uint32_t* y = &v[x / 16][2 * (x % 16)];
             const float2 e = fma2(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), make_float2(c2, c2), make_float2(neg, neg));
-            const float2 pp = make_float2(ex2(e.x), ex2(e.y));
-            sum[x & 1] = add2(sum[x & 1], pp);
-            const __nv_bfloat162 hh = __floats2bfloat162_rn(pp.x, pp.y);
+            const __nv_bfloat162 hh = __floats2bfloat162_rn(ex2(e.x), ex2(e.y));
             p[x] = *reinterpret_cast<const uint32_t*>(&hh);
+            // (the sum is of the rounded weights, which the values get: a row of one large weight has no error of it)
+            sum[x & 1] = add2(sum[x & 1], make_float2(__uint_as_float(p[x] << 16), __uint_as_float(p[x] & 0xffff0000u)));
           }
           tmem_st_32x32(at, p);
           sum[0] = add2(sum[0], sum[1]);
@@ -378,7 +379,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
             if (there)
 #pragma unroll
               for (int x = 0; x < 32; x += 4)
-                *reinterpret_cast<float4*>(a.part_o + at * D + c + x) = make_float4(__uint_as_float(o[x]), __uint_as_float(o[x + 1]),
+                if (c + x < a.D) *reinterpret_cast<float4*>(a.part_o + at * a.D + c + x) = make_float4(__uint_as_float(o[x]), __uint_as_float(o[x + 1]),
                                                                                   __uint_as_float(o[x + 2]), __uint_as_float(o[x + 3]));
           }
         }
@@ -410,8 +411,9 @@ static inline bool make_kv_map(CUtensorMap* out, const Args& a, int box) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// (internal linkage: what it keeps must not be one with that of another library built from this file)
 template <int D, int RING>
-int launch_tc(const Args& a, cudaStream_t stream) {
+static int launch_tc(const Args& a, cudaStream_t stream) {
   static_assert(RING % 2 == 0 && RING <= TC_MAX_RING, "the ring's barriers");
   constexpr size_t smem = (size_t)(2 + 2 * RING) * (D / 64) * TC_TILE + sizeof(TcCtl) + sizeof(Plan);
   static_assert(smem <= 227 * 1024, "shared memory of a block");

@@ -340,6 +340,20 @@ def test_attention_prefix_does_not_follow_bad_indices(dtype):
     assert torch.equal(starts[:4], good[:4]) and err.item() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_prefix_beside_its_bounds_check_build(dtype):
+    """Both builds' libraries in one process, each with state of its own."""
+    from sglang_c_b200.csrc import build
+    c = prefix_case([(300, [(9, 1)] * 5)], 4, 2, 64, 16, dtype, seed=9)
+    first = _run_prefix(c)
+    build.set_bounds_check(True)
+    try:
+        assert torch.equal(_run_prefix(c), first)
+    finally:
+        build.set_bounds_check(False)
+    assert torch.equal(_run_prefix(c), first)
+
+
 def test_attention_prefix_beyond_32_bits():
     """Pages whose offset in the cache passes 2^31 and 2^32 elements."""
     n_pages, page, Hkv, D = 70000, 64, 4, 128
