@@ -280,7 +280,8 @@ prefix_own_kernel(const Args a) {
   const bool inside = g >= 0 && t >= t0 && t < t1;
   // (starts that do not ascend, with the token behind this group's end and before the last one's)
   if (g >= 0 && !inside && t < min(a.group_start[a.G], a.T)) flag_index(a);
-  const int keys = inside ? prefix_length(a, g) : 0, walker = (share * WARPS + warp % WARPS) * per_warp + of_warp;
+  int keys = inside ? prefix_length(a, g) : 0;           // of the prefix, by parts; own keys lie behind them
+  const int walker = (share * WARPS + warp % WARPS) * per_warp + of_warp;
   const int walkers = WARPS * shares * per_warp, d = sub * 8;
   const bool cols = d < D;
   State st[HC];
@@ -293,8 +294,13 @@ prefix_own_kernel(const Args a) {
   }
   if (inside) {
     const float c2 = a.scale * LOG2E;
-    const int pos = a.positions[t], req = request_of(a, t);
+    const int pos = a.positions[t];
+    int req = request_of(a, t);
     if (pos > a.last_position) flag_index(a);
+    if (!sees_all(pos, keys)) {                        // inside the prefix, whose pages the group's first request names
+      keys = 0;
+      req = request_of(a, t0);
+    }
     const int end = req < 0 ? keys : min(pos, a.last_position) + 1;          // own keys: keys .. end - 1
     float2 q[HC][4];
 #pragma unroll

@@ -66,8 +66,12 @@ __device__ __forceinline__ size_t row_at(const Args& a, int page, int hk, int ke
   return (((size_t)page * 2 * a.Hkv + hk) * a.page_size + (key - block_in(a, key) * a.page_size)) * a.D;
 }
 __device__ __forceinline__ size_t value_offset(const Args& a) { return (size_t)a.Hkv * a.page_size * a.D; }
-// keys of a prefix of `keys` that token t sees
-__device__ __forceinline__ int visible(const Args& a, int t, int keys) { return min(keys, max(a.positions[t], -1) + 1); }
+// A token inside a prefix of `keys` sees only its first ones, and is the second launch's with all of them: in a tile that
+// rows beside it see further into, the first would give it weights of 0 times values that it must not see, which are no
+// zeros where those are infinite or no numbers.
+__device__ __forceinline__ bool sees_all(int position, int keys) { return position >= keys - 1; }
+// keys of a prefix of `keys` that token t gets from the first launch
+__device__ __forceinline__ int visible(const Args& a, int t, int keys) { return sees_all(a.positions[t], keys) ? keys : 0; }
 
 // A group's tokens and how many keys of its prefix there are.
 __device__ __forceinline__ void group_tokens(const Args& a, int g, int& t0, int& t1) {

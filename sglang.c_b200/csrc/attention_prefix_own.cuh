@@ -11,6 +11,8 @@
 // columns does not matter as long as queries and keys agree; and of the values, whose 8 x 8 pieces are transposed in
 // registers, a lane ends with eight neighbouring columns of a row of sums, as the parts and the results lie in memory.
 #pragma once
+#include <type_traits>
+
 #include "attention_prefix.cuh"
 
 namespace prefix {
@@ -69,6 +71,10 @@ prefix_join_kernel(const Args a, int tokens, int heads) {
       if (pos > a.last_position || r < 0 || r >= a.R) flag_index(a);
       hi = min(pos, a.last_position) + 1;
       req = r >= 0 && r < a.R ? r : -1;
+      if (!sees_all(pos, lo)) {                        // inside the prefix, whose pages the group's first request names
+        lo = 0;
+        req = request_of(a, t0);
+      }
     } else if (tl < end) {
       flag_index(a);                                   // starts that do not ascend
     }
@@ -116,108 +122,152 @@ prefix_join_kernel(const Args a, int tokens, int heads) {
 #pragma unroll
       for (int i = 0; i < 4; i++) o[b][j][i] = 0.0f;
   const size_t v_at = value_offset(a);
-  // one request after the other (their tokens need not stand together)
-  unsigned todo = __ballot_sync(0xffffffffu, inside && req >= 0 && hi > lo);
-  while (todo) {
-    const int who = __shfl_sync(0xffffffffu, req, __ffs(todo) - 1);
-    const unsigned same = __ballot_sync(0xffffffffu, inside && req == who) & todo;
-    todo &= ~same;
-    const bool mine = same >> lane & 1;
-    const int first = __reduce_min_sync(0xffffffffu, mine ? lo : 0x7fffffff), last = __reduce_max_sync(0xffffffffu, mine ? hi : 0);
-    int from[2], to[2];
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-      const bool here = row_in[x] && (same >> (row_token[x] & 31) & 1);
-      from[x] = here ? row_lo[x] : 0x7fffffff;
-      to[x] = here ? row_hi[x] : 0;
-    }
-    int block0 = -64, id = -1;                         // 32 pages at a time, a lane an id
-    for (long long key_at = first + 16LL * walker; key_at < last; key_at += 16LL * walkers) {
-      const int key0 = (int)key_at;
-      uint4 kv[2][2][B];                               // [keys g, g + 8][keys, values][block]
-      const int page_block = block_in(a, key0), top_block = block_in(a, min(key0 + 15, last - 1));
-      if (top_block >= block0 + 32 || page_block < block0) {
-        block0 = page_block;
-        id = (long long)(block0 + lane) * a.page_size < last ? page_of(a, who, (block0 + lane) * a.page_size) : -1;
-      }
+  // A tile's rows do not see the same keys, and a weight of 0 times an infinite value, or one that is no number, is no number:
+  // where the sums end with such, the walk is done again, with the values row by row as that row sees them.
+  auto walk = [&](auto row_by_row) {
+    // one request after the other (their tokens need not stand together)
+    unsigned todo = __ballot_sync(0xffffffffu, inside && req >= 0 && hi > lo);
+    while (todo) {
+      const int who = __shfl_sync(0xffffffffu, req, __ffs(todo) - 1);
+      const unsigned same = __ballot_sync(0xffffffffu, inside && req == who) & todo;
+      todo &= ~same;
+      const bool mine = same >> lane & 1;
+      const int first = __reduce_min_sync(0xffffffffu, mine ? lo : 0x7fffffff), last = __reduce_max_sync(0xffffffffu, mine ? hi : 0);
+      int from[2], to[2];
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-        const int key = key0 + 8 * x + g, block = block_in(a, key);
-        const int page = __shfl_sync(0xffffffffu, id, (block - block0) & 31);
-        const bool there = key < last && page >= 0;
-        const T* src = reinterpret_cast<const T*>(a.cache) +
-                       (((size_t)(there ? page : 0) * 2 * a.Hkv + hk) * a.page_size + (there ? key - block * a.page_size : 0)) * D + 8 * q;
+        const bool here = row_in[x] && (same >> (row_token[x] & 31) & 1);
+        from[x] = here ? row_lo[x] : 0x7fffffff;
+        to[x] = here ? row_hi[x] : 0;
+      }
+      int block0 = -64, id = -1;                         // 32 pages at a time, a lane an id
+      for (long long key_at = first + 16LL * walker; key_at < last; key_at += 16LL * walkers) {
+        const int key0 = (int)key_at;
+        uint4 kv[2][2][B];                               // [keys g, g + 8][keys, values][block]
+        const int page_block = block_in(a, key0), top_block = block_in(a, min(key0 + 15, last - 1));
+        if (top_block >= block0 + 32 || page_block < block0) {
+          block0 = page_block;
+          id = (long long)(block0 + lane) * a.page_size < last ? page_of(a, who, (block0 + lane) * a.page_size) : -1;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const int key = key0 + 8 * x + g, block = block_in(a, key);
+          const int page = __shfl_sync(0xffffffffu, id, (block - block0) & 31);
+          const bool there = key < last && page >= 0;
+          const T* src = reinterpret_cast<const T*>(a.cache) +
+                         (((size_t)(there ? page : 0) * 2 * a.Hkv + hk) * a.page_size + (there ? key - block * a.page_size : 0)) * D + 8 * q;
+#pragma unroll
+          for (int b = 0; b < B; b++) {
+            kv[x][0][b] = kv[x][1][b] = make_uint4(0u, 0u, 0u, 0u);
+            if (there) {
+              kv[x][0][b] = *reinterpret_cast<const uint4*>(src + 32 * b);
+              kv[x][1][b] = *reinterpret_cast<const uint4*>(src + v_at + 32 * b);
+            }
+          }
+        }
+        float s[2][4];                                   // scores: [keys 0..7, 8..15][row g: keys 2 q, 2 q + 1; row g + 8]
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[x][i] = 0.0f;
+#pragma unroll
+          for (int b = 0; b < B; b++) {
+            mma_16816(s[x], qf[b][0], kv[x][0][b].x, kv[x][0][b].y);
+            mma_16816(s[x], qf[b][1], kv[x][0][b].z, kv[x][0][b].w);
+          }
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int key = key0 + 8 * x + 2 * q + (i & 1);
+            s[x][i] = key >= from[i >> 1] && key < to[i >> 1] ? s[x][i] * c2 : -INFINITY;
+            top[i >> 1] = fmaxf(top[i >> 1], s[x][i]);
+          }
+        bool moved = false;
+        float f[2], ref[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+          top[x] = fmaxf(top[x], m[x]);
+          ref[x] = top[x] == -INFINITY ? 0.0f : top[x];
+          f[x] = ex2(m[x] - ref[x]);
+          moved |= top[x] > m[x];
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            l[x] *= f[x];
+            m[x] = top[x];
+          }
+#pragma unroll
+          for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) o[b][j][i] *= f[i >> 1];
+        }
+        uint32_t p[4];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          // (sums of the rounded weights, which the values get)
+#pragma unroll
+          for (int y = 0; y < 2; y++) {
+            const uint32_t w = pack_bf16(ex2(s[x][2 * y] - ref[y]), ex2(s[x][2 * y + 1] - ref[y]));
+            l[y] += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
+            p[2 * x + y] = w;
+          }
+        }
 #pragma unroll
         for (int b = 0; b < B; b++) {
-          kv[x][0][b] = kv[x][1][b] = make_uint4(0u, 0u, 0u, 0u);
-          if (there) {
-            kv[x][0][b] = *reinterpret_cast<const uint4*>(src + 32 * b);
-            kv[x][1][b] = *reinterpret_cast<const uint4*>(src + v_at + 32 * b);
+          const uint32_t v0[4] = {kv[0][1][b].x, kv[0][1][b].y, kv[0][1][b].z, kv[0][1][b].w};
+          const uint32_t v1[4] = {kv[1][1][b].x, kv[1][1][b].y, kv[1][1][b].z, kv[1][1][b].w};
+          if constexpr (!decltype(row_by_row)::value) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) mma_16816(o[b][j], p, transposed(v0[j]), transposed(v1[j]));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll 1
+              for (int i = 0; i < 8; i++) {              // row i + 8 x, which lanes 4 i .. 4 i + 3 have
+                const int begin = __shfl_sync(0xffffffffu, from[x], 4 * i), end = __shfl_sync(0xffffffffu, to[x], 4 * i);
+                const bool see0 = key0 + g >= begin && key0 + g < end, see1 = key0 + 8 + g >= begin && key0 + 8 + g < end;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                  float one[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                  mma_16816(one, p, transposed(see0 ? v0[j] : 0u), transposed(see1 ? v1[j] : 0u));
+                  if (g == i) {
+                    o[b][j][2 * x] += one[2 * x];
+                    o[b][j][2 * x + 1] += one[2 * x + 1];
+                  }
+                }
+              }
           }
         }
       }
-      float s[2][4];                                   // scores: [keys 0..7, 8..15][row g: keys 2 q, 2 q + 1; row g + 8]
+    }
+  };
+  walk(std::false_type());
+  if (tokens > 1) {
+    float number = 0.0f;
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
+    for (int b = 0; b < B; b++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[x][i] = 0.0f;
+      for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int b = 0; b < B; b++) {
-          mma_16816(s[x], qf[b][0], kv[x][0][b].x, kv[x][0][b].y);
-          mma_16816(s[x], qf[b][1], kv[x][0][b].z, kv[x][0][b].w);
-        }
-      }
-      float top[2] = {-INFINITY, -INFINITY};
+        for (int i = 0; i < 4; i++) number = fmaf(o[b][j][i], 0.0f, number);
+    if (__any_sync(0xffffffffu, number != number)) {
 #pragma unroll
-      for (int x = 0; x < 2; x++)
+      for (int x = 0; x < 2; x++) m[x] = -INFINITY, l[x] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int key = key0 + 8 * x + 2 * q + (i & 1);
-          s[x][i] = key >= from[i >> 1] && key < to[i >> 1] ? s[x][i] * c2 : -INFINITY;
-          top[i >> 1] = fmaxf(top[i >> 1], s[x][i]);
-        }
-      bool moved = false;
-      float f[2], ref[2];
+      for (int b = 0; b < B; b++)
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        top[x] = fmaxf(top[x], m[x]);
-        ref[x] = top[x] == -INFINITY ? 0.0f : top[x];
-        f[x] = ex2(m[x] - ref[x]);
-        moved |= top[x] > m[x];
-      }
-      if (__any_sync(0xffffffffu, moved)) {
+        for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          l[x] *= f[x];
-          m[x] = top[x];
-        }
-#pragma unroll
-        for (int b = 0; b < B; b++)
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[b][j][i] *= f[i >> 1];
-      }
-      uint32_t p[4];
-#pragma unroll
-      for (int x = 0; x < 2; x++) {
-        // (sums of the rounded weights, which the values get)
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-          const uint32_t w = pack_bf16(ex2(s[x][2 * y] - ref[y]), ex2(s[x][2 * y + 1] - ref[y]));
-          l[y] += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
-          p[2 * x + y] = w;
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < B; b++) {
-        const uint32_t v0[4] = {kv[0][1][b].x, kv[0][1][b].y, kv[0][1][b].z, kv[0][1][b].w};
-        const uint32_t v1[4] = {kv[1][1][b].x, kv[1][1][b].y, kv[1][1][b].z, kv[1][1][b].w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) mma_16816(o[b][j], p, transposed(v0[j]), transposed(v1[j]));
-      }
+          for (int i = 0; i < 4; i++) o[b][j][i] = 0.0f;
+      walk(std::true_type());
     }
   }
 #pragma unroll

@@ -818,7 +818,8 @@ def attention_prefix(q, cache, block_table, token_req, positions, group_start, s
     0..shared_len[g]-1 (int32 [G]; 0: none).  These are read once for all tokens of the group, through the row of
     block_table ([R, width], row stride free) of its first token's request; the keys behind them through each token's
     own row.  Token t belongs to request token_req[t] (None: to the t-th) and sees the keys of positions 0..positions[t]
-    (so one that lies inside the prefix sees its part of it; a position below 0 sees nothing and gives zeros).  A request
+    (so one that lies inside the prefix sees its part of it, read for it alone; a position below 0 sees nothing and gives
+    zeros).  A key or value that is infinite or no number is in the results that see it and in no other.  A request
     may bring any number of tokens; their keys and values are in the cache.  Tokens before group_start[0] or from
     group_start[G] on are left out: their rows of out stay as they were.
 

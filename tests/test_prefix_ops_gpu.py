@@ -196,6 +196,31 @@ def test_attention_prefix_rows_that_see_little(dtype):
     assert bool((out[0] == 0).all())
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("H,Hkv,D", [(2, 2, 64), (8, 2, 128), (4, 4, 136)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_prefix_of_keys_that_are_no_numbers(dtype, H, Hkv, D, which, value):
+    """A key (which 0) or value (1) that is no number or infinite, in the prefix and among a request's own: it is in the
+    rows that see it and leaves all others as they are."""
+    base = prefix_case([(150, [(4, 3), (2, 2), (0, 4), (1, 1)]), (0, [(3, 5)])], H, Hkv, D, 16, dtype, seed=5)
+    base["pos"][5:7] = torch.tensor([80, 149])                # (inside the prefix; its last key)
+    base["pos"][8] = -1
+    exact = prefix_exact(base)
+    # (request, position): in the prefix; a request's own; the last position of another; another group's
+    for r, p in [(0, 100), (0, 155), (2, 153), (4, 4)]:
+        c = dict(base, cache=base["cache"].clone())
+        pages = [int(c["table"][r, p // 16])] if p >= 150 or r == 4 else [int(x) for x in c["table"][:4, p // 16].unique()]
+        for page in pages:
+            c["cache"][page, which, :, p % 16, 5] = value
+        sees = (c["pos"] >= p) & ((c["req"] == r) if p >= 150 or r == 4 else (c["req"] < 4))
+        out = _run_prefix(c).double().cpu()
+        off = (out - exact[0]).abs() - prefix_bound(c, exact)
+        assert bool((off[~sees] <= 0).all()), (r, p)
+        if which or value != value:                           # (an infinite key may be a weight of 0)
+            assert not bool(torch.isfinite(out[sees].view(-1, H, D)[..., 5]).any()), (r, p)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_prefix_strided_rows_and_padded_batches(dtype):
     """Queries and results as columns of wider rows, off 16 bytes; rows before the first group and behind the last one stay."""
