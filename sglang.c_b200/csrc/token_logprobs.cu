@@ -126,7 +126,7 @@ struct Shared {
   float group[64];                        // maxima of groups of threads
   float seg[SEGMENTS][THREADS];           // a thread's maxima of stretches of its turns
   int chosen[SEGMENTS * THREADS];         // (stretch, thread)
-  int n_chosen, n_above, n_out;
+  int n_chosen, n_above;
   float threshold;
   unsigned long long above[ROOM];
   unsigned long long list[MAX_TOP];       // the block's best, in order

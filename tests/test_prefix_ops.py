@@ -66,6 +66,19 @@ def test_step_tables_refuses_one_word_for_both_counts(host):
         _tables(n_free=n, left=n)
 
 
+def test_step_tables_refuses_what_it_reads_as_what_it_writes(host):
+    x, words, tokens = _i32(20), _i32(2), _i32(20)
+    for kw in (dict(q_len=x[:3], q_start=x[:4]), dict(n_free=words[:1], status=words[:1]), dict(left=words[:1], status=words[:1]),
+               dict(kv_len=tokens[:3], positions=tokens), dict(slots=tokens, positions=tokens)):
+        with pytest.raises(ops.KernelError, match="other memory"):
+            _tables(**kw)
+    none = _i32(0)
+    with pytest.raises(host):                              # (arrays without entries are no memory)
+        _tables(q_len=none, kv_len=none, new_len=none, token_req=none, positions=none, slots=none)
+    with pytest.raises(host):                              # (what is only read may be one array)
+        _tables(q_len=x[:3], kv_len=x[:3])
+
+
 def _prefix(**kw):
     a = dict(q=torch.zeros(5, 48), cache=torch.zeros(7, 2, 2, 4, 8), block_table=_i32(3, 4), token_req=_i32(5), positions=_i32(5),
              group_start=_i32(3), shared_len=_i32(2), out=torch.zeros(5, 48), n_heads=6, scale=0.3)
