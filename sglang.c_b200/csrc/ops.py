@@ -388,14 +388,15 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
         raise KernelError("step_tables: n_free, left and status are one word each")
     if int(page_size) != page_size or not 0 < page_size <= 1 << 20:
         raise KernelError(f"step_tables: page size {page_size}")
-    read = (q_len.data_ptr(), kv_len.data_ptr(), free_pages.data_ptr(), n_free.data_ptr())
-    start, after, req, pos, slot, n_after, word = written = (q_start.data_ptr(), new_len.data_ptr(), token_req.data_ptr(),
-                                                             positions.data_ptr(), slots.data_ptr(), left.data_ptr(), status.data_ptr())
-    apart = {*written} - {0}                                                   # (0: an array without entries)
-    if len(apart) + written.count(0) < len(written) or not apart.isdisjoint(read):
-        raise KernelError("step_tables: an array that is written must be other memory than the others")
+    new, held, free, n, start, after, req, pos, slot, n_after, word = (
+        q_len.data_ptr(), kv_len.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), q_start.data_ptr(), new_len.data_ptr(),
+        token_req.data_ptr(), positions.data_ptr(), slots.data_ptr(), left.data_ptr(), status.data_ptr())
+    if len({new, held, free, n, start, after, req, pos, slot, n_after, word}) < 11:
+        read, written = (new, held, free, n), [p for p in (start, after, req, pos, slot, n_after, word) if p]    # (0: no entries)
+        if len({*written}) < len(written) or not {*written}.isdisjoint(read):
+            raise KernelError("step_tables: an array that is written must be other memory than the others")
     lib, fn = _function("step_tables", "sglc_step_tables", "pppippqiiippppp" "ipp" "p")
-    code = fn(read[0], read[1], read[2], free_pages.numel(), read[3], block_table.data_ptr(), pitch, width, R, int(page_size), start,
+    code = fn(new, held, free, free_pages.numel(), n, block_table.data_ptr(), pitch, width, R, int(page_size), start,
               after, req, pos, slot, T, n_after, word, _stream_here(here))
     _check(lib, code, "step_tables")
 
