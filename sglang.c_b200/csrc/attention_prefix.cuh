@@ -41,6 +41,7 @@ struct Plan {
   int t0[MAX_GROUPS], keys[MAX_GROUPS], rows[MAX_GROUPS];
   int items[MAX_GROUPS + 1];
   long long tiles[MAX_GROUPS + 1];
+  long long at, end;                      // this block's share of the tiles
 };
 
 __device__ __forceinline__ void flag_index(const Args& a) {
@@ -89,6 +90,32 @@ __device__ __forceinline__ long long divide(long long x, int y) {
   return (unsigned long long)x >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
 }
 
+// All tiles, items one after the other, go to the blocks in equal shares: block b has the tiles from b * tiles / blocks on, and
+// no share is empty.  Such shares end inside items, and a piece of an item costs a block its start (queries, first keys) and its end
+// (sums out to the workspace) beside its tiles, about as much as PIECE tiles.  So where that is less, blocks take whole items, from b *
+// items / blocks on.  (144 items of 12 tiles for 148 blocks: in shares of 11.7 a call takes 49.6 us, whole 45.4; 25 of 64 tiles
+// stay with shares.)
+constexpr int PIECE = 3;
+__device__ __forceinline__ void take_share(const Args& a, Plan& p, int items, long long tiles, int longest) {
+  // (a warp; the rule in floats, the same ones in every block: every block waits for this)
+  const int blocks = (int)min((long long)a.n_blocks, tiles), x = blockIdx.x + (threadIdx.x & 1);      // its share's start and end
+  long long at = 0;
+  if (tiles > 0 && (int)blockIdx.x < blocks) {
+    const float each = __fdividef(1.0f, (float)blocks), share = ceilf((float)tiles * each), n = (float)longest;
+    const float pieces = share < 2.0f ? 1.0f : 2.0f + floorf(__fdividef(share - 2.0f, n));             // (at most)
+    if (ceilf((float)items * each) * (n + PIECE) >= share + PIECE * pieces) {
+      at = divide(tiles * x, blocks);
+    } else {
+      const int takers = min(blocks, items), item = (int)divide((long long)items * min(x, takers), takers);
+      int g = 0;
+      for (; p.items[g + 1] < item; g++) {
+      }
+      at = p.tiles[g] + (long long)(item - p.items[g]) * tiles_of_keys(a, p.keys[g]);
+    }
+  }
+  if (threadIdx.x < 2) (threadIdx.x ? p.end : p.at) = at;
+}
+
 // Every thread of the block calls it.
 __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
   for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
@@ -103,12 +130,14 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
   }
   __syncthreads();
   if (threadIdx.x < 32) {                 // sums over the groups before
-    int items = 0;
+    int items = 0, longest = 0;
     long long tiles = 0;
     for (int g0 = 0; g0 < a.G; g0 += 32) {
       const int g = g0 + threadIdx.x;
       int x = g < a.G ? p.items[g + 1] : 0;
-      long long y = g < a.G ? (long long)x * tiles_of_keys(a, p.keys[g]) : 0;
+      const int kt = x > 0 ? tiles_of_keys(a, p.keys[g]) : 0;
+      long long y = (long long)x * kt;
+      longest = max(longest, __reduce_max_sync(0xffffffffu, kt));
       for (int o = 1; o < 32 && o < a.G; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, x, o);
         const long long v = __shfl_up_sync(0xffffffffu, y, o);
@@ -126,13 +155,11 @@ __device__ __forceinline__ void make_plan(const Args& a, Plan& p) {
       tiles += __shfl_sync(0xffffffffu, y, last);
     }
     if (threadIdx.x == 0) p.items[0] = 0, p.tiles[0] = 0;
+    __syncwarp();
+    take_share(a, p, items, tiles, longest);
   }
   __syncthreads();
 }
-
-// All tiles, items one after the other, go to `blocks` blocks in equal shares: block b has the tiles from b * tiles / blocks
-// on.  No share is empty.
-__device__ __forceinline__ int blocks_used(const Args& a, long long tiles) { return (int)min((long long)a.n_blocks, tiles); }
 
 // A block's piece of an item.
 struct Segment {
@@ -166,12 +193,7 @@ __device__ __forceinline__ Segment segment_at(const Args& a, const Plan& p, long
   s.row0 = (n - s.hk * rt) << s.shift;
   return s;
 }
-__device__ __forceinline__ Segment first_segment(const Args& a, const Plan& p) {
-  const long long tiles = p.tiles[a.G];
-  const int blocks = blocks_used(a, tiles);
-  if ((int)blockIdx.x >= blocks) return segment_at(a, p, 0, 0);
-  return segment_at(a, p, divide(tiles * blockIdx.x, blocks), divide(tiles * (blockIdx.x + 1), blocks));
-}
+__device__ __forceinline__ Segment first_segment(const Args& a, const Plan& p) { return segment_at(a, p, p.at, p.end); }
 __device__ __forceinline__ Segment next_segment(const Args& a, const Plan& p, const Segment& s) {
   return segment_at(a, p, s.at + s.tiles, s.end);
 }

@@ -366,21 +366,40 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
         tc_fence_after_sync();
       }
       if (threadIdx.x == 0) record_item(a, s);
-      if (busy && ok) {
+      if (__all_sync(0xffffffffu, ok) && busy) {
         const long long at = (long long)(blockIdx.x + s.item) * TC_SLOT + (pair ? 0 : w * TC_WG) + mine;
         const bool there = valid && slot_ok(a, s);
         if (there) a.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * c2, l);
         if (steps > 0) {
+          // More than 64 rows (32 of two blocks of columns) go out by way of where the queries were, so that eight lanes store 128 bytes side by side: a thread a row, 16
+          // bytes of 32 rows a store, took 2.6 us for 256 rows of 64 and 5.5 for rows of 128 (96 rows of 96, a whole call: 26.1 us,
+          // 23.8 this way; 64 rows of 128: 23.5 and 22.9).  Of fewer rows a store reaches few lines, and the way round is the longer one (a
+          // whole call with 8 rows of 64: 56.3 us, 57.6 this way; with 64: 39.4 and 39.9).
+          uint8_t* turn_at = sQ + w * UNIT + (warp & 3) * 32 * 128;
+          const unsigned rows_there = __ballot_sync(0xffffffffu, there);
+          const long long at0 = at - lane;           // (a warp's rows lie side by side in the slot)
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32(tO + c, o);
             tmem_ld_wait();
-            if (there)
+            if (rows * DB > 64) {
 #pragma unroll
               for (int x = 0; x < 32; x += 4)
-                if (c + x < a.D) *reinterpret_cast<float4*>(a.part_o + at * a.D + c + x) = make_float4(__uint_as_float(o[x]), __uint_as_float(o[x + 1]),
-                                                                                  __uint_as_float(o[x + 2]), __uint_as_float(o[x + 3]));
+                *reinterpret_cast<uint4*>(turn_at + sw128(lane, x / 4)) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+              __syncwarp();
+#pragma unroll
+              for (int x = 0; x < 8; x++) {
+                const int r = 4 * x + (lane >> 3), k = lane & 7;
+                if ((rows_there >> r & 1) && c + 4 * k < a.D)
+                  *reinterpret_cast<uint4*>(a.part_o + (at0 + r) * a.D + c + 4 * k) = *reinterpret_cast<const uint4*>(turn_at + sw128(r, k));
+              }
+              __syncwarp();
+            } else if (there) {
+#pragma unroll
+              for (int x = 0; x < 32; x += 4)
+                if (c + x < a.D) *reinterpret_cast<uint4*>(a.part_o + at * a.D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            }
           }
         }
       }

@@ -186,6 +186,14 @@ def test_attention_prefix_long(dtype, H, Hkv, D, prefix, own):
         _check_prefix(c, _run_prefix(c, max_own=max_own), exact)
 
 
+@pytest.mark.parametrize("H,Hkv,D", [(150, 150, 8), (149, 149, 64), (100, 100, 128), (296, 148, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_prefix_of_whole_items(dtype, H, Hkv, D):
+    """About as many items as blocks, of more tiles than one, beside groups without tokens or prefix: blocks take whole items."""
+    c = prefix_case([(0, [(3, 1)]), (64, []), (900, [(2, 1)] * 2), (640, []), (1000, [(0, 1), (9, 2)]), (0, [])], H, Hkv, D, 16, dtype, seed=H + D)
+    _check_prefix(c, _run_prefix(c))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_prefix_rows_that_see_little(dtype):
     """Tokens inside the prefix see their part of it; one at position -1 sees nothing."""
