@@ -248,34 +248,37 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
       const int lim = valid ? visible(a, t, s.keys) : 0;
       // both groups are done with the item before (its products have been waited for): queries of this one
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      // (all 256 threads, pieces of 16 bytes side by side: a thread a row took 12,000 cycles for 256 rows of 128; eight asked
-      // for at a time)
-      for (int x0 = threadIdx.x; x0 < (D / 8) << s.shift; x0 += 8 * 2 * TC_WG) {
-        uint4 x[8];
+      // (all 256 threads, pieces of 16 bytes side by side: a thread a row took 12,000 cycles for 256 rows of 128; four asked for
+      // at a time, and rows off 16 bytes in a loop of their own: the less code there is to fetch, the sooner a block begins)
+      auto query = [&](int at) {                     // where piece `at` lies, or null: zeros
+        const int r = at / (D / 8), c = at % (D / 8), nr = s.row0 + r, tr = (unsigned)nr / (unsigned)gq;
+        const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(s.t0 + tr) * a.q_stride + (size_t)(s.hk * gq + nr - tr * gq) * a.D + c * 8;
+        return r < rows && c * 8 < a.D ? from : nullptr;
+      };
+      auto put = [&](int at, uint4 x) {
+        const int r = at / (D / 8), c = at % (D / 8);
+        uint8_t* to = sQ + (c / 8) * TC_TILE;
+        *reinterpret_cast<uint4*>(to + (r / TC_WG) * UNIT + sw128(r % TC_WG, c % 8)) = x;
+        if (!pair) *reinterpret_cast<uint4*>(to + UNIT + sw128((r + 64) & (TC_WG - 1), c % 8)) = x;
+      };
+      const int pieces = (D / 8) << s.shift;         // (a multiple of 4 for each thread)
+      if (a.q_vec) {
+        for (int x0 = threadIdx.x; x0 < pieces; x0 += 4 * 2 * TC_WG) {
+          uint4 x[4];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int at = x0 + u * 2 * TC_WG, r = at / (D / 8), c = at % (D / 8);
-          x[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows && c * 8 < a.D) {
-            const int nr = s.row0 + r, tr = (unsigned)nr / (unsigned)gq;
-            const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)(s.t0 + tr) * a.q_stride + (size_t)(s.hk * gq + nr - tr * gq) * a.D + c * 8;
-            if (a.q_vec) {
-              x[u] = *reinterpret_cast<const uint4*>(from);
-            } else {
-              const unsigned short* h = reinterpret_cast<const unsigned short*>(from);
-              x[u] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                                h[6] | (uint32_t)h[7] << 16);
-            }
+          for (int u = 0; u < 4; u++) {
+            const __nv_bfloat16* from = query(x0 + u * 2 * TC_WG);
+            x[u] = from ? *reinterpret_cast<const uint4*>(from) : make_uint4(0u, 0u, 0u, 0u);
           }
+#pragma unroll
+          for (int u = 0; u < 4; u++) put(x0 + u * 2 * TC_WG, x[u]);
         }
-#pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int at = x0 + u * 2 * TC_WG, r = at / (D / 8), c = at % (D / 8);
-          if (r < 1 << s.shift) {
-            uint8_t* to = sQ + (c / 8) * TC_TILE;
-            *reinterpret_cast<uint4*>(to + (r / TC_WG) * UNIT + sw128(r % TC_WG, c % 8)) = x[u];
-            if (!pair) *reinterpret_cast<uint4*>(to + UNIT + sw128((r + 64) & (TC_WG - 1), c % 8)) = x[u];
-          }
+      } else {
+#pragma unroll 1
+        for (int at = threadIdx.x; at < pieces; at += 2 * TC_WG) {
+          const unsigned short* h = reinterpret_cast<const unsigned short*>(query(at));
+          put(at, h ? make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16)
+                    : make_uint4(0u, 0u, 0u, 0u));
         }
       }
       fence_async_proxy();
@@ -375,30 +378,37 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
           // bytes of 32 rows a store, took 2.6 us for 256 rows of 64 and 5.5 for rows of 128 (96 rows of 96, a whole call: 26.1 us,
           // 23.8 this way; 64 rows of 128: 23.5 and 22.9).  Of fewer rows a store reaches few lines, and the way round is the longer one (a
           // whole call with 8 rows of 64: 56.3 us, 57.6 this way; with 64: 39.4 and 39.9).
-          uint8_t* turn_at = sQ + w * UNIT + (warp & 3) * 32 * 128;
-          const unsigned rows_there = __ballot_sync(0xffffffffu, there);
-          const long long at0 = at - lane;           // (a warp's rows lie side by side in the slot)
+          if (rows * DB <= 64) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32(tO + c, o);
-            tmem_ld_wait();
-            if (rows * DB > 64) {
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(tO + c, o);
+              tmem_ld_wait();
+              if (there)
+#pragma unroll
+                for (int x = 0; x < 32; x += 4)
+                  if (c + x < a.D) *reinterpret_cast<uint4*>(a.part_o + at * a.D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            }
+          } else {
+            uint8_t* turn_at = sQ + w * UNIT + (warp & 3) * 32 * 128;
+            const unsigned rows_there = __ballot_sync(0xffffffffu, there);
+            const long long at0 = at - lane;           // (a warp's rows lie side by side in the slot)
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(tO + c, o);
+              tmem_ld_wait();
 #pragma unroll
               for (int x = 0; x < 32; x += 4)
                 *reinterpret_cast<uint4*>(turn_at + sw128(lane, x / 4)) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
               __syncwarp();
-#pragma unroll
+#pragma unroll 2
               for (int x = 0; x < 8; x++) {
                 const int r = 4 * x + (lane >> 3), k = lane & 7;
                 if ((rows_there >> r & 1) && c + 4 * k < a.D)
                   *reinterpret_cast<uint4*>(a.part_o + (at0 + r) * a.D + c + 4 * k) = *reinterpret_cast<const uint4*>(turn_at + sw128(r, k));
               }
               __syncwarp();
-            } else if (there) {
-#pragma unroll
-              for (int x = 0; x < 32; x += 4)
-                if (c + x < a.D) *reinterpret_cast<uint4*>(a.part_o + at * a.D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
             }
           }
         }
