@@ -209,7 +209,7 @@ prefix_general_kernel(const Args a) {
 // own with a running maximum of its own, then, once the first launch is done, parts of the prefix in the same way.  Walkers
 // meet by shuffles, warps in shared memory, blocks through the cluster's.  What bounds it: the keys' and the parts' way from
 // memory, and for few items the chain token -> request -> page -> key; so a lane of the warp holds a page's id each, and the
-// keys of a round are asked for together.
+// keys of a round are asked for together.  (64 requests of 25 heads of 64 with 300 keys each: 22 us alone, 123 MB.)
 constexpr int OT = 128;
 
 constexpr int OWN_ONE = 16, OWN_TWO = 4;    // items a multiprocessor from which an item has one warp, two

@@ -103,7 +103,8 @@ __device__ __forceinline__ void take_share(const Args& a, Plan& p, int items, lo
   if (tiles > 0 && (int)blockIdx.x < blocks) {
     const float each = __fdividef(1.0f, (float)blocks), share = ceilf((float)tiles * each), n = (float)longest;
     const float pieces = share < 2.0f ? 1.0f : 2.0f + floorf(__fdividef(share - 2.0f, n));             // (at most)
-    if (ceilf((float)items * each) * (n + PIECE) >= share + PIECE * pieces) {
+    // (a part of a round is 1 / 296 or more: what the reciprocal's rounding adds is none)
+    if (ceilf((float)items * each - 1e-3f) * (n + PIECE) >= share + PIECE * pieces) {
       at = divide(tiles * x, blocks);
     } else {
       const int takers = min(blocks, items), item = (int)divide((long long)items * min(x, takers), takers);

@@ -5,7 +5,7 @@
 // (where requests bring several, most of them share their keys).  A warp takes 16 keys at a time on the warp-level
 // tensor-core instruction: 16 x 16 scores, their weights as bfloat16, 16 x D sums.  (tcgen05 would want 128 rows; here a
 // few rows meet keys that nobody else reads, and what bounds it is instructions and the keys' way from memory: on
-// multiply-adds, 1,961 tokens of 16 heads with 30 keys each took 50 us.)
+// multiply-adds, 1,961 tokens of 16 heads with 30 keys each took 50 us, this way 14.)
 // Operands come from global memory straight into the instruction's registers, 16 bytes a lane: with lane = 4 g + q, a lane
 // holds of key g the columns 8 q .. 8 q + 7 of each block of 32.  Which column is called which along the sum over
 // columns does not matter as long as queries and keys agree; and of the values, whose 8 x 8 pieces are transposed in

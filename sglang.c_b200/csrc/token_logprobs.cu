@@ -6,10 +6,14 @@
 // The row is read once: a thread keeps (m, s, w) of the entries it meets, sixteen at a time, scaled to its running maximum,
 // and the place is a count of those few sixteens that reach the token's logit.  The best k come from the threads'
 // maxima: k groups of threads have a maximum of T or more for T the k-th largest of the groups', so the best k are T or more,
-// and they lie in the few stretches of a thread's turns whose own maximum is: only those (a hundredth of the row,
-// still in L2) are looked at again.
+// and they lie in the few stretches of a thread's turns whose own maximum is: only those (an eighth of a thread's
+// entries each, for about 31 threads at k = 20: a sixtieth of the row, still in L2) are looked at again.
 // Sums are 32-bit, a thread's over V / 256 entries and then pairwise.  The exponential is the special-function unit's
 // (2 ulp) of a difference taken exactly as it is rounded, so no logit is too large for it.
+// What bounds it on a B200: float32, the logits' way from memory and the last rows' blocks (2,048 rows of 50,257: 82 us, 4.9 TB/s);
+// bfloat16, instructions, half of whose bytes bring twice the entries (777 rows of 128,000: 63 us, 3.2 TB/s, the exponentials alone
+// 22); few rows, what follows the pass (64 rows with 20 best 13 us, one row 7).  Blocks of 256 threads, four a multiprocessor: with 512
+// or 1,024 a row's end, where threads wait for one another, was the longer.
 #include "common.cuh"
 
 SGLC_DEFINE_ERROR_STRING()
