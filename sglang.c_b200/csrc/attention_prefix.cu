@@ -622,8 +622,8 @@ SGLC_API int sglc_attention_prefix(const void* q, long long q_stride, const void
   if (!sizes_ok(T, R, G, H, Hkv, D) || page_size <= 0 || n_pages < 0 || bt_width < 0 || !(scale > 0.0f) ||
       (dtype != SGLC_F32 && dtype != SGLC_BF16))
     return SGLC_ERR_ARGUMENT;
-  if (D % 8 || D > 256 || G > MAX_GROUPS || (long long)T * H > 0x7fffffffLL || T > 0x1fffffff || n_pages == 0 ||
-      ((uintptr_t)cache & 15))
+  // (items of all groups are counted in 32 bits, also where starts do not ascend and groups overlap)
+  if (D % 8 || D > 256 || G > MAX_GROUPS || (long long)T * H > 0x20000000LL || n_pages == 0 || ((uintptr_t)cache & 15))
     return SGLC_ERR_UNSUPPORTED;
   if (T == 0 || G == 0) return SGLC_OK;
   Args a = {};

@@ -841,8 +841,8 @@ def attention_prefix(q, cache, block_table, token_req, positions, group_start, s
     if q.dim() != 2 or out.dim() != 2:
         raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
     (T, q_width), (q_pitch, q_column), (rows, width), (pitch, column) = q.shape, q.stride(), out.shape, out.stride()
-    if T > _MOST or cache.numel() == 0:
-        raise KernelError(f"attention_prefix: {T} tokens (at most {_MOST}), a cache of {n_pages} pages of {page_size}")
+    if T * n_heads > _MOST or cache.numel() == 0:
+        raise KernelError(f"attention_prefix: {T} tokens of {n_heads} heads (at most {_MOST} rows), a cache of {n_pages} pages of {page_size}")
     if q_width != n_heads * D or width != q_width or rows < T or q_column != 1 or column != 1:
         raise KernelError("attention_prefix: query/output rows do not match heads x head_dim")
     if rows > 1 and pitch < width:

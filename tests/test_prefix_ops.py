@@ -173,6 +173,8 @@ def test_sizes_beyond_32_bits_are_refused(host):
             _logprobs(logits=logits)
     with pytest.raises(ops.KernelError, match="at most 536870912"):
         _prefix(q=torch.empty((1 << 30, 48), device="meta"))
+    with pytest.raises(ops.KernelError, match="100000000 tokens of 6 heads .at most 536870912"):
+        _prefix(q=torch.empty((100000000, 48), device="meta"))
     with pytest.raises(ops.KernelError, match="at most 16384 and 536870912"):
         _tables(token_req=torch.empty(1 << 30, dtype=torch.int32, device="meta"))
     with pytest.raises(ops.KernelError, match="a cache of 0 pages"):
