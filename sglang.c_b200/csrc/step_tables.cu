@@ -28,6 +28,12 @@ struct Args {
   int vec;                                // the tokens' arrays begin on 16 bytes
 };
 
+// What the warps find of their runs of requests.
+struct Warps {
+  long long q[THREADS / 32], p[THREADS / 32];
+  int bad[THREADS / 32];
+};
+
 // the last r of 0..n-1 with first[r] <= x (first ascends; requests without any share their successor's start)
 __device__ __forceinline__ int find(const int* first, int n, int x) {
   int lo = 0, hi = n;                     // first[lo] <= x < first[hi]
@@ -45,8 +51,7 @@ step_tables_kernel(const Args a) {
   int* start = sm;                        // [R + 1]: lengths first, then first tokens
   int* taken = sm + R + 1;                // [R + 1]: pages that the requests before take
   int* kv = sm + 2 * (R + 1);             // [R]
-  __shared__ long long warp_q[THREADS / 32], warp_p[THREADS / 32];
-  __shared__ int warp_bad[THREADS / 32];
+  __shared__ Warps warps;
   // (The arrays written here are what later kernels of a step read ahead of their own wait, so this kernel lets none
   // of them begin before it ends: there is no early release of dependents.)
   pdl_wait();
@@ -82,9 +87,9 @@ step_tables_kernel(const Args a) {
   }
   bad = __reduce_or_sync(0xffffffffu, (unsigned)bad);
   if (lane == 31) {
-    warp_q[warp] = q_run;
-    warp_p[warp] = p_run;
-    warp_bad[warp] = bad;
+    warps.q[warp] = q_run;
+    warps.p[warp] = p_run;
+    warps.bad[warp] = bad;
   }
   __syncthreads();
   long long q_all = 0, p_all = 0, q_before = 0, p_before = 0;
@@ -95,9 +100,9 @@ step_tables_kernel(const Args a) {
       q_before = q_all;
       p_before = p_all;
     }
-    q_all += warp_q[w];
-    p_all += warp_p[w];
-    bad |= warp_bad[w];
+    q_all += warps.q[w];
+    p_all += warps.p[w];
+    bad |= warps.bad[w];
   }
   if (n_free < 0 || n_free > a.free_cap) bad |= BAD_LENGTH;
   if (p_all > n_free) bad |= PAGES_SHORT;
@@ -193,7 +198,9 @@ SGLC_API int sglc_step_tables(const int* q_len, const int* kv_len, const int* fr
                   token_req, positions, slots, left, status,
                   (((uintptr_t)token_req | (uintptr_t)positions | (uintptr_t)slots) & 15) == 0};
   const size_t smem = (size_t)(3 * R + 2) * 4;
-  if (smem > 48 * 1024) {                 // (one value for all sizes: two threads may be here at once)
+  // The 48 KB that a block has without an attribute are for both kinds of shared memory, the kernel's own words too (from 4,069
+  // requests on).  One value for all sizes: two threads may be here at once.
+  if (smem + sizeof(Warps) > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (3 * MAX_REQUESTS + 2) * 4);
     if (e != cudaSuccess) return (int)e;

@@ -79,6 +79,25 @@ def test_step_tables_of_many_requests(R, most, context, page):
     assert torch.equal(got["table"][:R].cpu(), table) and bool((got["table"][R:] == -7).all())
 
 
+@pytest.mark.parametrize("R", [4068, 4069, 4095, 4096])
+def test_step_tables_where_shared_memory_needs_an_attribute(R, tmp_path, monkeypatch):
+    """About 48 KB of it, in a library loaded afresh: what an earlier call allowed the kernel would hide that this one does not."""
+    import ctypes
+    import shutil
+
+    from sglang_c_b200.csrc import build
+    build.load("step_tables")
+    lib = ctypes.CDLL(shutil.copy(build.lib_path("step_tables"), tmp_path / f"tables_{R}.so"))
+    lib.sglc_error_string.restype, lib.sglc_error_string.argtypes = ctypes.c_char_p, [ctypes.c_int]
+    monkeypatch.setitem(build._loaded, ("step_tables", False), lib)
+    got, want, args = _tables([i % 3 for i in range(R)], [i % 50 for i in range(R)], 16)
+    _run_tables(got, args)
+    T = len(want["req"])
+    assert got["status"].item() == 0 and got["left"].item() == want["left"] and got["q_start"].tolist() == want["start"] + [-9]
+    for name, row in (("token_req", want["req"]), ("positions", want["pos"]), ("slots", want["slot"])):
+        assert got[name].tolist() == row + [-9] * (got[name].numel() - T), name
+
+
 def test_step_tables_of_no_requests():
     got, want, args = _tables([], [], 16)
     _run_tables(got, args)
