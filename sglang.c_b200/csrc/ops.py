@@ -353,6 +353,8 @@ def _here(what, *tensors):
 
 
 STEP_TABLES_REQUESTS = 16384     # requests step_tables takes (step_tables.cu: MAX_REQUESTS)
+_STEP_TABLES_OVERLAP = -4        # its launcher's code for arrays that overlap (step_tables.cu: OVERLAP)
+_STEP_TABLES_APART = "step_tables: an array that is written must be other memory than the others"
 
 
 def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_start, new_len, token_req, positions, slots,
@@ -365,8 +367,8 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
     stay free) and status[0].  What the arrays hold behind the last token stays as it was.
 
     All or nothing: where the pages are too few (status 1), a row too short (2), the tokens more than the arrays hold (4)
-    or a length is out of range (8; sums of these), only status is written.  All arrays int32.  What is written lies apart
-    from what is read (every block reads all lengths): the lengths after a step become the next one's by turns."""
+    or a length is out of range (8; sums of these), only status is written.  All arrays int32.  What is written shares no memory
+    with anything else of the call (every block reads all lengths): the lengths after a step become the next one's by turns."""
     arrays = (q_len, kv_len, free_pages, n_free, q_start, new_len, token_req, positions, slots, left, status)
     here = _here("step_tables", block_table, *arrays)
     for t in arrays:
@@ -391,13 +393,15 @@ def step_tables(q_len, kv_len, free_pages, n_free, block_table, page_size, q_sta
     new, held, free, n, start, after, req, pos, slot, n_after, word = (
         q_len.data_ptr(), kv_len.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), q_start.data_ptr(), new_len.data_ptr(),
         token_req.data_ptr(), positions.data_ptr(), slots.data_ptr(), left.data_ptr(), status.data_ptr())
-    if len({new, held, free, n, start, after, req, pos, slot, n_after, word}) < 11:
+    if len({new, held, free, n, start, after, req, pos, slot, n_after, word}) < 11:       # (other overlaps: the launcher's look)
         read, written = (new, held, free, n), [p for p in (start, after, req, pos, slot, n_after, word) if p]    # (0: no entries)
         if len({*written}) < len(written) or not {*written}.isdisjoint(read):
-            raise KernelError("step_tables: an array that is written must be other memory than the others")
+            raise KernelError(_STEP_TABLES_APART)
     lib, fn = _function("step_tables", "sglc_step_tables", "pppippqiiippppp" "ipp" "p")
     code = fn(new, held, free, free_pages.numel(), n, block_table.data_ptr(), pitch, width, R, int(page_size), start,
               after, req, pos, slot, T, n_after, word, _stream_here(here))
+    if code == _STEP_TABLES_OVERLAP:
+        raise KernelError(_STEP_TABLES_APART)
     _check(lib, code, "step_tables")
 
 

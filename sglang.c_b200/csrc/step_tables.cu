@@ -17,6 +17,7 @@ SGLC_DEFINE_ERROR_STRING()
 namespace {
 constexpr int THREADS = 512;
 constexpr int MAX_REQUESTS = 16384;       // three words each in shared memory
+constexpr int OVERLAP = -4;               // (a launcher's code: what is written lies in what is read)
 enum { PAGES_SHORT = 1, ROW_SHORT = 2, TOKENS_MANY = 4, BAD_LENGTH = 8 };
 
 struct Args {
@@ -182,11 +183,55 @@ step_tables_kernel(const Args a) {
   }
   __threadfence();                        // (see above: readers that do not wait begin once every block has ended)
 }
+
+// `words` words from `at` on.
+struct Span {
+  const int* at;
+  long long words;
+  bool meets(const Span& x) const {
+    const uintptr_t p = (uintptr_t)at, q = (uintptr_t)x.at;
+    return words > 0 && x.words > 0 && p < q + 4 * (uintptr_t)x.words && q < p + 4 * (uintptr_t)words;
+  }
+};
+// Whether what a call may write shares words with anything else of it.  (Every block reads all lengths, and none waits for
+// another: block 0 would change them under those that begin later.  Of the table only its rows count, not what lies between.)
+bool overlaps(const Args& a) {
+  const Span read[] = {{a.q_len, a.R}, {a.kv_len, a.R}, {a.free_pages, a.free_cap}, {a.n_free, 1}};
+  const Span written[] = {{a.q_start, a.R + 1LL}, {a.new_len, a.R}, {a.token_req, a.t_cap}, {a.positions, a.t_cap}, {a.slots, a.t_cap},
+                          {a.left, 1}, {a.status, 1}};
+  auto in_table = [&](const Span& x) {
+    const uintptr_t base = (uintptr_t)a.table, end = (uintptr_t)x.at + 4 * (uintptr_t)x.words;
+    if (x.words <= 0 || a.R <= 0 || a.bt_width <= 0 || end <= base) return false;
+    // the last row that begins before its end
+    const uintptr_t pitch = 4 * (uintptr_t)(a.bt_stride > 0 ? a.bt_stride : 1), last = (end - 1 - base) / pitch, rows = (uintptr_t)a.R - 1;
+    const Span row = {a.table + (long long)(last < rows ? last : rows) * a.bt_stride, a.bt_width};
+    return row.meets(x);
+  };
+  for (const Span& x : read)
+    if (in_table(x)) return true;
+  for (const Span& x : written) {
+    if (in_table(x)) return true;
+    for (const Span& y : read)
+      if (x.meets(y)) return true;
+    for (const Span& y : written)
+      if (&x < &y && x.meets(y)) return true;
+  }
+  return false;
+}
 }  // namespace
+
+// Whether arrays of a call overlap as sglc_step_tables does not take them (1 or 0); no memory is touched.
+SGLC_API int sglc_step_tables_overlap(const int* q_len, const int* kv_len, const int* free_pages, int free_cap, const int* n_free,
+                                      int* table, long long bt_stride, int bt_width, int R, int* q_start, int* new_len,
+                                      int* token_req, int* positions, int* slots, int t_cap, int* left, int* status) {
+  const Args a = {q_len, kv_len, free_pages, n_free, table, bt_stride, bt_width, free_cap, R, 1, t_cap, q_start, new_len,
+                  token_req, positions, slots, left, status, 0};
+  return overlaps(a);
+}
 
 // All arrays int32.  table [R][bt_stride], bt_width entries a row; free_pages: a stack of free_cap words of which the
 // first *n_free are free pages, the top last; t_cap: room for tokens in token_req, positions, slots.  What
-// is written lies apart from what is read.  *status: 0, or why nothing was written: 1 too few pages, 2 a table row too
+// is written lies apart from all else (-4 where it does not).  *status: 0, or why nothing was written: 1 too few pages, 2 a table row too
 // short, 4 more tokens than t_cap, 8 a length below zero or beyond 2^31, or n_free outside the stack.
 SGLC_API int sglc_step_tables(const int* q_len, const int* kv_len, const int* free_pages, int free_cap, const int* n_free,
                               int* table, long long bt_stride, int bt_width, int R, int page_size, int* q_start, int* new_len,
@@ -197,6 +242,7 @@ SGLC_API int sglc_step_tables(const int* q_len, const int* kv_len, const int* fr
   const Args a = {q_len, kv_len, free_pages, n_free, table, bt_stride, bt_width, free_cap, R, page_size, t_cap, q_start, new_len,
                   token_req, positions, slots, left, status,
                   (((uintptr_t)token_req | (uintptr_t)positions | (uintptr_t)slots) & 15) == 0};
+  if (overlaps(a)) return OVERLAP;
   const size_t smem = (size_t)(3 * R + 2) * 4;
   // The 48 KB that a block has without an attribute are for both kinds of shared memory, the kernel's own words too (from 4,069
   // requests on).  One value for all sizes: two threads may be here at once.

@@ -79,6 +79,51 @@ def test_step_tables_refuses_what_it_reads_as_what_it_writes(host):
         _tables(q_len=x[:3], kv_len=x[:3])
 
 
+_SPANS = dict(q_len=(0, 5), kv_len=(10, 5), free_pages=(20, 9), n_free=(30, 1), table=(100, 0), q_start=(40, 6), new_len=(50, 5),
+              token_req=(60, 8), positions=(70, 8), slots=(80, 8), left=(90, 1), status=(92, 1))
+
+
+def _overlap(stride=7, width=4, R=5, **at):
+    """The launcher's look at arrays at made-up addresses (words from 2^20 on; nothing is read)."""
+    import ctypes
+    p = {k: ctypes.c_void_p((1 << 20) + 4 * at.get(k, v[0])) for k, v in _SPANS.items()}
+    return build.load("step_tables").sglc_step_tables_overlap(
+        p["q_len"], p["kv_len"], p["free_pages"], 9, p["n_free"], p["table"], ctypes.c_longlong(stride), width, R, p["q_start"],
+        p["new_len"], p["token_req"], p["positions"], p["slots"], 8, p["left"], p["status"])
+
+
+_READ = ("q_len", "kv_len", "free_pages", "n_free")
+
+
+def test_step_tables_overlaps_word_by_word():
+    """Every written array against every other one: overlap by a word at either end, and side by side."""
+    assert _overlap() == 0
+    names = [n for n in _SPANS if n != "table"]
+    for a in names:
+        for b in names:
+            if a == b:
+                continue
+            far = {a: 1000}                                  # (a clear of the rest, b moved along it)
+            size_a, size_b = _SPANS[a][1], _SPANS[b][1]
+            for start in (1000 - size_b, 1000 - size_b + 1, 1000, 1000 + size_a - 1, 1000 + size_a):
+                meets = start + size_b > 1000 and start < 1000 + size_a
+                want = int(meets and not (a in _READ and b in _READ))
+                assert _overlap(**far, **{b: start}) == want, (a, b, start)
+
+
+def test_step_tables_overlaps_with_the_table():
+    """An array in one of the table's rows, each word of it; between rows (7 words apart, 4 of them the row's) there is room for one."""
+    inside = {100 + 7 * r + i for r in range(5) for i in range(4)}
+    for name, (_, size) in _SPANS.items():
+        if name == "table":
+            continue
+        for start in range(85, 150):
+            want = int(any(w in inside for w in range(start, start + size)))
+            others = {n: 2000 + 50 * i for i, n in enumerate(_SPANS) if n not in (name, "table")}
+            assert _overlap(**{**others, name: start}) == want, (name, start)
+    assert _overlap(R=0, table=40) == 0 and _overlap(width=0, table=50) == 0        # (no rows, or rows without entries)
+
+
 def _prefix(**kw):
     a = dict(q=torch.zeros(5, 48), cache=torch.zeros(7, 2, 2, 4, 8), block_table=_i32(3, 4), token_req=_i32(5), positions=_i32(5),
              group_start=_i32(3), shared_len=_i32(2), out=torch.zeros(5, 48), n_heads=6, scale=0.3)

@@ -122,6 +122,23 @@ def test_step_tables_write_all_or_nothing(change, status):
         assert k == "status" or torch.equal(v, before[k]), k
 
 
+def test_step_tables_refuse_arrays_that_overlap():
+    """Lengths read and written at one word's distance, and an array inside the table; nothing is written."""
+    ops = _ops()
+    got, want, args = _tables([2, 1, 3], [15, 16, 30], 16)
+    x, before = _i32([15, 16, 30, 7, 7]), {k: v.clone() for k, v in got.items()}
+    for kw in (dict(args, kv_len=x[:3]), dict(args, q_len=x[:3]), dict(args, free_pages=got["table"].view(-1)[:9])):
+        out = {k: v for k, v in got.items() if k != "table"}
+        if "kv_len" in kw and kw["kv_len"].data_ptr() == x.data_ptr():
+            out["new_len"] = x[1:4]
+        if kw["q_len"].data_ptr() == x.data_ptr():
+            out["q_start"] = x[1:]
+        with pytest.raises(ops.KernelError, match="other memory"):
+            ops.step_tables(**kw, **out)
+    torch.cuda.synchronize()
+    assert x.tolist() == [15, 16, 30, 7, 7] and all(torch.equal(v, before[k]) for k, v in got.items())
+
+
 def test_step_tables_in_a_graph_follow_the_lengths():
     """A captured call replayed after the lengths, the stack and the table have changed."""
     got, want, args = _tables([1, 2, 3], [15, 16, 30], 16, width=6)
