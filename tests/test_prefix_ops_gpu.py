@@ -230,6 +230,102 @@ def test_attention_prefix_of_whole_items(dtype, H, Hkv, D):
     _check_prefix(c, _run_prefix(c))
 
 
+# (type, key heads, query heads of each, size, tokens a request): those the joining kernel of 16 rows an item takes, and the others
+JOINED = [(torch.bfloat16, 2, 4, 64, 1), (torch.bfloat16, 2, 8, 128, 1), (torch.bfloat16, 12, 1, 64, 9), (torch.bfloat16, 8, 1, 128, 9),
+          (torch.bfloat16, 3, 5, 64, 9), (torch.bfloat16, 2, 20, 64, 1)]
+BY_HEADS = [(torch.bfloat16, 12, 1, 64, 1), (torch.bfloat16, 6, 2, 128, 1), (torch.bfloat16, 4, 4, 40, 1), (torch.float32, 12, 1, 64, 1),
+            (torch.float32, 6, 2, 64, 3), (torch.float32, 4, 4, 128, 1)]
+
+
+def _tokens_where_forms_change(Hkv, gq, tokens, joined):
+    """Numbers of tokens just below and from where an item has two warps of its own, and one (by the rules' own constants)."""
+    import os
+    import re
+
+    from sglang_c_b200.csrc import ops
+    here, sms = os.path.dirname(ops.__file__), torch.cuda.get_device_properties(DEV).multi_processor_count
+
+    def constant(name, word):
+        with open(os.path.join(here, name)) as f:
+            return int(re.search(rf"{word} = (\d+)", f.read()).group(1))
+    if joined:
+        file, words, each = "attention_prefix_own.cuh", ("JOIN_TWO", "JOIN_ONE"), Hkv * ((gq + 15) // 16)
+        of_item = max(n for n in (1, 2, 4, 8, 16) if n == 1 or n * gq <= 16 and n <= tokens)
+    else:
+        file, words, of_item = "attention_prefix.cu", ("OWN_TWO", "OWN_ONE"), 1
+        each = Hkv * gq // (4 if gq % 4 == 0 else 2 if gq % 2 == 0 else 1)
+    at = [(-(-constant(file, w) * sms // each) - 1) * of_item + 1 for w in words]          # the first token of the item that does it
+    return [(n, form) for a, forms in zip(at, ((4, 2), (2, 1))) for n, form in zip((a - 1, a + 2), forms)]
+
+
+def _many_tokens(n, dtype, Hkv, gq, D, tokens, seed):
+    """n tokens in groups of three kinds, with counts a request about `tokens`; some tokens inside a prefix, one that sees nothing."""
+    counts, kinds = [], (1,) if tokens == 1 else (tokens - 2, tokens + 3, tokens, tokens + 1, tokens - 1)
+    while sum(counts) < n:
+        counts.append(min(kinds[len(counts) % len(kinds)], n - sum(counts)))
+    requests = [(i % 7, c) for i, c in enumerate(counts)]
+    a, b = len(requests) // 4, len(requests) // 2
+    c = prefix_case([(0, requests[:a]), (70, requests[a:b]), (64, []), (33, requests[b:])], Hkv * gq, Hkv, D, 16, dtype, seed=seed)
+    second = int(c["start"][1])
+    c["pos"][second + 1:second + 4] = torch.tensor([-1, 5, 68])
+    return c
+
+
+@pytest.mark.parametrize("step", range(4))
+@pytest.mark.parametrize("kind", JOINED + BY_HEADS)
+def test_attention_prefix_of_many_items(kind, step):
+    """Enough items that one has two warps, or one, and a block several items, with a last block that is partly empty; results
+    on 16 bytes and off them."""
+    dtype, Hkv, gq, D, tokens = kind
+    n, _ = _tokens_where_forms_change(Hkv, gq, tokens, kind in JOINED)[step]
+    c = _many_tokens(n, dtype, Hkv, gq, D, tokens, seed=n + D)
+    c["start"][0] = 1
+    c["start"][-1] = n - 1
+    exact = prefix_exact(c)
+    _check_prefix(c, _run_prefix(c), exact)
+    wide = torch.full((n, Hkv * gq * D + 11), 77.0, dtype=dtype, device=DEV)
+    out = wide[:, 3:3 + Hkv * gq * D]
+    _check_prefix(c, _run_prefix(c, out=out), exact)
+    assert bool((wide[:, :3] == 77.0).all()) and bool((wide[:, 3 + Hkv * gq * D:] == 77.0).all())
+
+
+@pytest.mark.parametrize("step", [1, 3])
+@pytest.mark.parametrize("kind", [JOINED[0], JOINED[2], JOINED[4], BY_HEADS[0], BY_HEADS[4]])
+def test_attention_prefix_of_many_items_with_values_that_are_no_numbers(kind, step):
+    """Such a value among each fourth request's own: in the rows that see it, and in none of the others that share its item."""
+    dtype, Hkv, gq, D, tokens = kind
+    n, _ = _tokens_where_forms_change(Hkv, gq, tokens, kind in JOINED)[step]
+    base = _many_tokens(n, dtype, Hkv, gq, D, tokens, seed=n)
+    exact = prefix_exact(base)
+    c = dict(base, cache=base["cache"].clone())
+    sees = torch.zeros(n, dtype=torch.bool)
+    group = torch.bucketize(torch.arange(n), base["start"][1:].long(), right=True)
+    for r in range(0, len(base["table"]), 4):
+        mine = (base["req"] == r).nonzero()[:, 0]
+        p = int(base["pos"][mine].max())                      # (its last token's key)
+        if p < int(base["shared"][group[mine[0]]]):
+            continue
+        c["cache"][int(base["table"][r, p // 16]), 1, :, p % 16, 3] = float("nan")
+        sees[mine] = base["pos"][mine] >= p
+    out = _run_prefix(c).double().cpu()
+    off = (out - exact[0]).abs() - prefix_bound(base, exact)
+    assert int(sees.sum()) > n // (5 * tokens) and bool((off[~sees] <= 0).all())
+    assert not bool(torch.isfinite(out[sees].view(-1, Hkv * gq, D)[..., 3]).any())
+
+
+@pytest.mark.parametrize("rows", [100, 1024])
+@pytest.mark.parametrize("kind", [JOINED[0], JOINED[2], BY_HEADS[3]])
+def test_attention_prefix_with_rows_of_the_table_that_no_token_has(kind, rows):
+    """A table with a row for every request that a server could hold, in any order; its rows choose the form of the second launch."""
+    dtype, Hkv, gq, D, tokens = kind
+    c = _many_tokens(40 * tokens, dtype, Hkv, gq, D, tokens, seed=rows)
+    where = torch.randperm(rows, generator=torch.Generator().manual_seed(rows))[:len(c["table"])]
+    table = torch.full((rows, c["table"].shape[1]), -1, dtype=torch.int32)
+    table[where] = c["table"]
+    c = dict(c, table=table, req=where[c["req"].long()].int())
+    _check_prefix(c, _run_prefix(c))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_prefix_rows_that_see_little(dtype):
     """Tokens inside the prefix see their part of it; one at position -1 sees nothing."""
