@@ -9,7 +9,11 @@
 // that key head), so keys serve rows from shared memory; the tiles of keys of all items, one after the other, are dealt to
 // the blocks in equal shares, so a block's share may end inside an item and every block has the same work, whatever the
 // lengths.  What a block finds for (a piece of) an item goes to the workspace.  The second launch makes the tokens' own parts,
-// which it does while the first still runs, waits for that, and joins all parts of a (token, head).
+// waits for the first, and joins all parts of a (token, head).  Its blocks may begin once all of the first's have, but find
+// room only where those leave it: on the tensor cores a block takes 61,440 of a multiprocessor's 65,536 registers.  So with
+// items for some multiprocessors only the two run side by side (8 requests of 12 heads on 512 keys: all own keys are done before the
+// first launch's last sums are out), and with items for all of them the second's blocks begin as the first's end (64 of 25 heads on
+// 8,192 keys: from 16 us on, the first's last sums are out at 20, and 18 of 800 blocks are done with their own keys by then).
 #include "attention_prefix.cuh"
 #include "attention_prefix_own.cuh"
 #include "attention_prefix_tc.cuh"
@@ -209,7 +213,7 @@ prefix_general_kernel(const Args a) {
 // own with a running maximum of its own, then, once the first launch is done, parts of the prefix in the same way.  Walkers
 // meet by shuffles, warps in shared memory, blocks through the cluster's.  What bounds it: the keys' and the parts' way from
 // memory, and for few items the chain token -> request -> page -> key; so a lane of the warp holds a page's id each, and the
-// keys of a round are asked for together.  (64 requests of 25 heads of 64 with 300 keys each: 22 us alone, 123 MB.)
+// keys of a round are asked for together.  (64 requests of 25 heads of 64 with up to 300 keys: 26 us alone, 62 MB.)
 constexpr int OT = 128;
 
 constexpr int OWN_ONE = 16, OWN_TWO = 4;    // items a multiprocessor from which an item has one warp, two
@@ -541,7 +545,9 @@ int launch_own(const Args& a, int shares, cudaStream_t stream) {
 template <typename T, int HC, int LW>
 int warps_own(const Args& a, int max_own, cudaStream_t stream) {
   // A warp an item where the items fill the multiprocessors' warps, else two, else four, and blocks of a cluster while
-  // there are fewer than four a multiprocessor and 64 keys or more are left for each.
+  // there are fewer than four a multiprocessor and 64 keys or more are left for each.  (By the items' number: the host knows no
+  // lengths.  Where one request has many more keys of its own than the others, its items' warps walk them alone: 256 requests of 25
+  // heads of 64 on 1,024 keys with 150 of their own take 73 us, with one of them at 3,000 259 us, at 30,000 2,120.)
   const long long items = (long long)a.T * (a.H / HC);
   if (items >= OWN_ONE * a.sms) return launch_own<T, HC, LW, 1>(a, 1, stream);
   if (items >= OWN_TWO * a.sms) return launch_own<T, HC, LW, 2>(a, 1, stream);

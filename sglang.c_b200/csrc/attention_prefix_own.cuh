@@ -5,7 +5,7 @@
 // (where requests bring several, most of them share their keys).  A warp takes 16 keys at a time on the warp-level
 // tensor-core instruction: 16 x 16 scores, their weights as bfloat16, 16 x D sums.  (tcgen05 would want 128 rows; here a
 // few rows meet keys that nobody else reads, and what bounds it is instructions and the keys' way from memory: on
-// multiply-adds, 1,961 tokens of 16 heads with 30 keys each took 50 us, this way 14.)
+// multiply-adds, 1,961 tokens of 16 heads with 30 keys each took 50 us, this way 16.)
 // Operands come from global memory straight into the instruction's registers, 16 bytes a lane: with lane = 4 g + q, a lane
 // holds of key g the columns 8 q .. 8 q + 7 of each block of 32.  Which column is called which along the sum over
 // columns does not matter as long as queries and keys agree; and of the values, whose 8 x 8 pieces are transposed in
@@ -412,7 +412,11 @@ int launch_join(const Args& a, int tokens, int heads, int shares, cudaStream_t s
   return sglc_launch(prefix_join_kernel<D, WARPS>, dim3((unsigned)((chunks * WARPS + 3) / 4), a.Hkv * ((a.gq + MR - 1) / MR), shares),
                      dim3(MT), smem, stream, shares, true, a, tokens, heads);
 }
-// Tokens an item: as many as fill 16 rows, where a request brings so many (as far as sizes tell: tokens a row of the table).
+// Tokens an item: as many as fill 16 rows, where a request brings so many.  As far as sizes tell, that is: the host knows tokens and
+// rows of the table, not which rows have tokens, nor how many each.  Rows that no token has make items smaller (69 requests of 28 tokens
+// of 16 heads of 64: 43 us with a table of 69 rows; with 1,024 an item is a token, the multiply-add kernel's, and the call takes
+// 77), and a long portion beside single tokens makes an item of those a walk over sixteen requests (900 tokens of a request 60 us, 60
+// requests of a token 27, both in a call 174).
 static inline int join_tokens(const Args& a) {
   const int heads = a.gq < MR ? a.gq : MR;
   int tokens = 1;

@@ -10,9 +10,13 @@
 //   rows of a group's key head <= 128: both groups have the same rows, and every other tile of keys each: what bounds it is
 //     the keys' way from memory, and a tile is met by 128 rows at most whatever is done;
 //   more: an item has 256 rows, 128 a group of warps, and each tile is met by both: half of the traffic for the same work.
-// What bounds it: with all rows filled the operands' way through shared memory (256 requests of 32 heads of 128 over 8 on 32,768 keys: 168
-// us alone, 0.82 PFLOP/s, the tensor pipe 40 % busy); else a step's exponentials and a warp's way through it (0.95 us for 64 keys of 256
-// rows, 0.55 of them the special-function units'), and 5 us until a block's first scores.
+// What bounds it: a row warp's way through a step of 64 keys, one thing after the other (wait, scores out of tensor memory, maximum,
+// exponentials, rounding, store, arrival) with one other row warp beside it on its scheduler.  Of the 1.06 us between two steps of
+// 256 rows of 64 it works 0.93, of 1.12 with rows of 128 0.96 to 0.99, of 0.8 with 64 rows 0.64, and waits 0.13 to 0.16 for products.  No
+// unit is what it waits for: 256 requests of 32 heads of 128 over 8 on 32,768 keys take 163 us alone, 0.85 PFLOP/s, with the tensor
+// pipe 42 % busy, the special-function units 44 % and the issue slots 43 %; without any exponentials the whole call fell from 187
+// to 180 us.  Ahead of that a block's first scores: the plan 1.0 to 1.4 us, queries to shared memory 1.4 (8 rows) to 6.9 (256 of 128), the first
+// keys and product 1 to 2.
 // Keys and values come page by page through the block table by TMA, in boxes of the largest power of two of rows that
 // divides the page, into a ring of tiles.  (No multicast.)
 #pragma once
@@ -352,9 +356,11 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap map_kv, const Args a, int b
         const int tile = tile_of(pair, w, i >> 1), in_tile = s.keys - (s.tile + tile) * TC_KEYS;
         if (in_tile < TC_KEYS && (i & 1) == 0) {
           // The end of the prefix: behind its last key a tile of values holds what the page or the ring held, which may be no
-          // number.  It becomes zeros, as the weights there are, before the weights are handed on.  (The tile that had this
-          // place in the ring before was this group's too, the ring being even, and behind a product that these scores came
-          // behind: so the parity tells this one's landing.  Where both groups take the tile both write the zeros.)
+          // number.  It becomes zeros, as the weights there are, before the weights are handed on.  (The parity tells this
+          // tile's landing, as the one that had its place in the ring before has landed: in the same piece it was this
+          // group's too, the ring being even, and behind a product that these scores came behind; a tile of an earlier piece may
+          // have been the other group's, but both groups waited for their last products of it ahead of the barrier above.  Where
+          // both groups take the tile both write the zeros.)
           const uint32_t u = u0 + tile, slot = u % RING;
           ok = mbar_wait(&ctl.full[1][slot], (u / RING) & 1, abort_flag);
           if (!ok) break;

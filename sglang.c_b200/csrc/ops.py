@@ -832,8 +832,14 @@ def attention_prefix(q, cache, block_table, token_req, positions, group_start, s
 
     q, out: [T, n_heads*head_dim] views, row stride free.  max_own: about how many keys of its own a token has, which only
     sizes the launch.  workspace: float32, attention_prefix_workspace() elements or more, used by this call alone
-    until it is done (None: taken from torch's allocator).  An index out of range (a request, a page, a position beyond the
-    table's row) is not followed and sets the error word (tc_error_flag)."""
+    until it is done (None: taken from torch's allocator).  It grows with groups x key heads, 256 rows of head_dim + 2 each in bfloat16
+    whether a group has the tokens or not (64 groups over 8 key heads of 128: 89 MB, 256 over 32: 1.1 GB).  An index out of
+    range (a request, a page, a position beyond the table's row) is not followed and sets the error word (tc_error_flag).
+
+    The launch is chosen by sizes: T over the rows of block_table is taken for the tokens that a request brings.  So the same
+    call with rows that no token has may take the slower form for few tokens a request (pass block_table[:n] where the step's requests
+    are its first n), and a token's bits may follow the number of tokens beside it (bfloat16 heads of 64 and 128: weights of own keys
+    are rounded to bfloat16 in one form, not in the other).  Every call with the same sizes gives the same bits."""
     here = _here("attention_prefix", q, cache, block_table, token_req, positions, group_start, shared_len, out, workspace)
     for t, nm in ((token_req, "token_req"), (positions, "positions"), (group_start, "group_start"), (shared_len, "shared_len")):
         if t is not None and (t.dtype is not _INT or not t.is_contiguous()):

@@ -7,9 +7,10 @@
 // All or nothing: lengths that do not fit set the status word and nothing else is written.
 //
 // What bounds it: a launch and a chain of dependent reads (lengths -> scan -> search -> page -> slot); the words written
-// are 12 bytes a token.  5 to 6 us a call in a row on a B200, for 64 requests of a token as for 260,000 tokens of 300.  One launch, no block waits for another: every block scans all requests' lengths (they are a few
-// kilobytes) into its own shared memory, and takes its share of the tokens and of the new pages, whose page it finds in
-// the free stack itself, without the table entry that another block writes.
+// are 12 bytes a token.  5 to 6 us a call in a row on a B200, for 64 requests of a token as for 260,000 tokens of 515.  One launch,
+// no block waits for another: every block scans all requests' lengths (they are a few kilobytes) into its own shared memory,
+// and takes its share of the tokens and of the new pages, whose page it finds in the free stack itself, without the table
+// entry that another block writes.
 #include "common.cuh"
 
 SGLC_DEFINE_ERROR_STRING()

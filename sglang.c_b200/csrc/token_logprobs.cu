@@ -11,9 +11,11 @@
 // Sums are 32-bit, a thread's over V / 256 entries and then pairwise.  The exponential is the special-function unit's
 // (2 ulp) of a difference taken exactly as it is rounded, so no logit is too large for it.
 // What bounds it on a B200: float32, the logits' way from memory and the last rows' blocks (2,048 rows of 50,257: 82 us, 4.9 TB/s);
-// bfloat16, instructions, half of whose bytes bring twice the entries (777 rows of 128,000: 63 us, 3.2 TB/s, the exponentials alone
-// 22); few rows, what follows the pass (64 rows with 20 best 13 us, one row 7).  Blocks of 256 threads, four a multiprocessor: with 512
-// or 1,024 a row's end, where threads wait for one another, was the longer.
+// bfloat16, no one thing (777 rows of 128,000: 63 us, 3.2 TB/s): twice the entries a byte keep the issue slots 64 % busy and the
+// special-function units 42 %, DRAM 39 %, a thread has two pieces of 16 bytes in flight where float32 has four, and 777 rows
+// are 1.3 rounds of 592 resident blocks; few rows, what follows the pass (64 rows with 20 best 13 us, one row 7).  A turn with a
+// forbidden entry (-inf) makes its exponentials twice, see there; the entropy's sums are made whether it is asked for or not.  Blocks of
+// 256 threads, four a multiprocessor: with 512 or 1,024 a row's end, where threads wait for one another, was the longer.
 #include "common.cuh"
 
 SGLC_DEFINE_ERROR_STRING()
@@ -309,8 +311,9 @@ token_logprobs_kernel(const Args a) {
   best = ranked(best);
 
   // ---- the block's sums and count (warp 0), and a threshold for its best k ----
-  // At least k entries reach the threshold: it is the k-th largest of the maxima of 32 (64) groups of threads.  About
-  // -32 ln(1 - k / 32) entries do (31 at k = 20), and so many threads at most have them.
+  // At least k entries reach the threshold: it is the k-th largest of the maxima of G = 32 (64) groups of threads.  In random
+  // order G (H_G - H_(G-k)) entries do on average, H_n = 1 + 1/2 + .. + 1/n: entries from the largest down until k groups have
+  // one (31 at k = 20, 130 at 32, 304 at 64), and so many threads at most have them.
   const int k = a.k, groups = k <= 32 ? 32 : 64, of_group = THREADS / groups;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {                 // (the warp's lanes have one reference)
